@@ -298,6 +298,82 @@ VELOGRAD_API int32_t velograd_rope(
     int64_t rot_dim, float theta, int32_t inverse, int32_t pairing,
     int32_t dtype, void* hip_stream);
 
+/*
+ * A paged cache of keys and values in the MX block formats of velograd_rmsnorm_residual_fwd_mx.  No
+ * counterpart in the reference's fused kernels.  All four arrays are bytes, 16-byte aligned:
+ *   codes  [pages, kv_heads, page_size, R]  R = head_dim / 2 (E2M1, the even element in the low nibble)
+ *          or head_dim (E4M3) bytes of a head vector
+ *   scales [pages, kv_heads, head_dim / 32, page_size]  E8M0 codes
+ * head_dim is 64, 128 or 256, page_size a power of two from 16 to 32768.  A token's slot is
+ * page * page_size + place.
+ *
+ * velograd_mx_cache_write quantises the keys and values of `tokens` new tokens into their slots (int64
+ * [tokens]); a slot outside the cache (-1, say) is not written.  Slots must differ: of two tokens with one
+ * slot, either may be kept, block by block.
+ *   k, v      : [tokens, kv_heads, head_dim] in `dtype`, unit stride along head_dim, any other strides (in
+ *               elements) and any element alignment.
+ *   positions : int64 [tokens], or NULL.  With positions, k is rotated (VELOGRAD_ROPE_HALF pairs over the
+ *               whole head_dim) by row positions[t] of cos_sin before it is quantised, and rounded to
+ *               `dtype` in between; q [tokens, q_heads, head_dim] (q_heads may be 0) is rotated into q_out
+ *               (contiguous, 16-byte aligned) by every token, slot or not.  Without, q_heads must be 0.
+ *   cos_sin   : fp32 [max_positions, head_dim] contiguous: head_dim / 2 cosines, then as many sines.  A
+ *               position outside the table rotates by NaN.
+ */
+VELOGRAD_API int32_t velograd_mx_cache_write(
+    const void* q, const void* k, const void* v, void* q_out, const float* cos_sin,
+    const int64_t* positions, const int64_t* slots,
+    void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+    int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+    int64_t v_token_stride, int64_t v_head_stride,
+    int64_t max_positions, int64_t pages, int64_t page_size, int32_t dtype, int32_t mx_format,
+    void* hip_stream);
+
+/*
+ * The keys and values of `tokens` slots (int64 [tokens], any order, repeats allowed) of the cache, as
+ * `dtype`: k, v [tokens, kv_heads, head_dim] contiguous, 16-byte aligned.  A slot outside the cache reads
+ * as zeros; blocks marked NaN read as NaN.
+ */
+VELOGRAD_API int32_t velograd_mx_cache_read(
+    const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+    const int64_t* slots, void* k, void* v,
+    int64_t tokens, int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
+    int32_t dtype, int32_t mx_format, void* hip_stream);
+
+/*
+ * Attention of new tokens over everything their sequences hold in the cache (the new tokens' own keys
+ * and values included: write them first).  Query head h reads kv head h / (q_heads / kv_heads).
+ *   q           : [q_tokens, q_heads, head_dim] in `dtype`, unit stride along head_dim, any other strides
+ *                 (in elements) and any element alignment.
+ *   block_table : int32 [sequences, table_width], row stride table_stride: the pages of each sequence in
+ *                 order.  Keys on a page outside the cache are not seen.
+ *   lengths     : int32 [sequences], tokens that each sequence holds (clamped to 0 .. table_width * page_size).
+ *   q_starts    : int32 [sequences + 1], rising from 0: sequence b's new tokens are rows q_starts[b] ..
+ *                 q_starts[b + 1] - 1 of q.  NULL: one for each sequence (q_tokens == sequences).
+ *   causal      : nonzero: the i-th of n new tokens of a sequence of L sees its first L - n + i + 1 keys;
+ *                 zero: all L.
+ *   out         : [q_tokens, q_heads, head_dim] in `dtype`, contiguous, 16-byte aligned.
+ *   lse         : fp32 [q_tokens, q_heads], log of the sum of exp(scale q.k) over the keys seen, or NULL.
+ * A row that sees no key, and a row of q that belongs to no sequence, gives out 0 and lse -inf.
+ *   workspace   : velograd_mx_cache_attention_workspace_bytes() bytes, 16-byte aligned (NULL if that is 0).
+ */
+VELOGRAD_API int32_t velograd_mx_cache_attention(
+    const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+    const void* v_scales, const int32_t* block_table, const int32_t* lengths,
+    const int32_t* q_starts, void* out, float* lse, void* workspace, size_t ws_bytes,
+    int64_t q_tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t table_stride, int64_t table_width,
+    int64_t pages, int64_t page_size, float scale, int32_t causal, int32_t dtype,
+    int32_t mx_format, void* hip_stream);
+
+/*
+ * Workspace of velograd_mx_cache_attention for a call of these sizes on `device`; `ragged` nonzero: with
+ * q_starts.  0 where none is needed, the arguments are invalid or the device cannot be queried.
+ */
+VELOGRAD_API size_t velograd_mx_cache_attention_workspace_bytes(
+    int64_t q_tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t table_width, int64_t page_size, int32_t ragged, int32_t device);
+
 /* Text of the calling thread's last error ("" if none).  No counterpart in the reference. */
 VELOGRAD_API const char* velograd_kernels_last_error(void);
 

@@ -135,6 +135,43 @@ SIGNATURES = {
          _c_i64, ctypes.c_float, _c_i32,    # rot_dim, theta, inverse
          _c_i32, _c_i32, _c_ptr],           # pairing, dtype, hip_stream
     ),
+    "velograd_mx_cache_write": (
+        _c_i32,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr,    # q, k, v, q_out
+         _c_ptr, _c_ptr, _c_ptr,            # cos_sin, positions, slots
+         _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # k_codes, k_scales, v_codes, v_scales
+         _c_i64, _c_i64, _c_i64, _c_i64,    # tokens, q_heads, kv_heads, head_dim
+         _c_i64, _c_i64, _c_i64, _c_i64,    # token and head strides of q, of k
+         _c_i64, _c_i64,                    # and of v
+         _c_i64, _c_i64, _c_i64,            # max_positions, pages, page_size
+         _c_i32, _c_i32, _c_ptr],           # dtype, mx_format, hip_stream
+    ),
+    "velograd_mx_cache_read": (
+        _c_i32,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr,    # k_codes, k_scales, v_codes, v_scales
+         _c_ptr, _c_ptr, _c_ptr,            # slots, k, v
+         _c_i64, _c_i64, _c_i64,            # tokens, kv_heads, head_dim
+         _c_i64, _c_i64,                    # pages, page_size
+         _c_i32, _c_i32, _c_ptr],           # dtype, mx_format, hip_stream
+    ),
+    "velograd_mx_cache_attention": (
+        _c_i32,
+        [_c_ptr,                            # q
+         _c_ptr, _c_ptr, _c_ptr, _c_ptr,    # k_codes, k_scales, v_codes, v_scales
+         _c_ptr, _c_ptr, _c_ptr,            # block_table, lengths, q_starts
+         _c_ptr, _c_ptr,                    # out, lse
+         _c_ptr, _c_size,                   # workspace, ws_bytes
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,  # q_tokens, sequences, q_heads, kv_heads, head_dim
+         _c_i64, _c_i64, _c_i64, _c_i64,    # token and head strides of q, table_stride, table_width
+         _c_i64, _c_i64, ctypes.c_float,    # pages, page_size, scale
+         _c_i32, _c_i32, _c_i32, _c_ptr],   # causal, dtype, mx_format, hip_stream
+    ),
+    "velograd_mx_cache_attention_workspace_bytes": (
+        _c_size,
+        [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64,  # q_tokens, sequences, q_heads, kv_heads, head_dim
+         _c_i64, _c_i64,                    # table_width, page_size
+         _c_i32, _c_i32],                   # ragged, device
+    ),
     "velograd_kernels_last_error": (ctypes.c_char_p, []),
     "velograd_kernels_version": (ctypes.c_char_p, []),
 }

@@ -15,7 +15,8 @@ import sys
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 # Translation units of the kernels library (one .so).
-SRCS = [os.path.join(PKG_DIR, "csrc", name) for name in ("rmsnorm_residual.hip", "rope.hip")]
+SRCS = [os.path.join(PKG_DIR, "csrc", name) for name in
+        ("rmsnorm_residual.hip", "rope.hip", "mx_cache.hip", "mx_attention.hip")]
 PROBE_SRC = os.path.join(PKG_DIR, "csrc", "stream_probe.hip")
 INCLUDE_DIR = os.path.join(REPO_DIR, "include")
 CSRC_DIR = os.path.join(PKG_DIR, "csrc")

@@ -32,7 +32,8 @@ gradient reaching h from the next residual add) to grad_x in the same pass.
 `fused_rmsnorm_residual_forward_fp8` returns y as fp8 E4M3 codes with one scale per row, and
 `fused_rmsnorm_residual_forward_mx` as MXFP8 / MXFP4 blocks (one E8M0 scale per 32 elements).
 `rmsnorm_forward` is the residual-free form of the reference's module (nn.py:338-355), with its
-floor on the mean square.
+floor on the mean square.  `mx_cache_write`, `rope_mx_cache_write`, `mx_cache_read` and
+`mx_cache_attention` (mx_cache.py) keep keys and values in those block formats and attend over them.
 """
 
 from __future__ import annotations
@@ -59,6 +60,13 @@ __all__ = [
     "fused_rope_backward",
     "fused_rope_interleaved",
     "bwd_workspace_bytes",
+    "MXCache",
+    "mx_cache",
+    "rope_table",
+    "mx_cache_write",
+    "rope_mx_cache_write",
+    "mx_cache_read",
+    "mx_cache_attention",
 ]
 
 
@@ -802,3 +810,8 @@ def fused_rmsnorm_residual(x: Any, residual: Optional[Any] = None, weight: Optio
                            eps: float = 1e-6):
     """Wrapper returning only the normalised output, like kernels/__init__.py:19-32."""
     return fused_rmsnorm_residual_forward(x, residual, weight, eps)[0]
+
+
+# The cache of keys and values in the MX formats.
+from .mx_cache import (MXCache, mx_cache, mx_cache_attention, mx_cache_read, mx_cache_write,  # noqa: E402
+                       rope_mx_cache_write, rope_table)
