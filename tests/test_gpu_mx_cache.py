@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from tests import _mx_cache as R
+from velograd_amd import _lib
 from velograd_amd import kernels as vk
 
 pytestmark = pytest.mark.gpu
@@ -15,6 +16,15 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 # each off by at most 2^-8 of what the parts before leave; two for 2-byte outputs, three for float32.
 OUT_EPS = {t: torch.finfo(t).eps / 2 for t in DTYPES.values()}
 P_EPS = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -16, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(autouse=True, params=["fast path", "general path"])
+def _path(request, monkeypatch):
+    """Every test through the C++ fast path and without it."""
+    if request.param == "general path":
+        monkeypatch.setattr(_lib, "fastpath", lambda: None)
+    else:
+        assert _lib.fastpath() is not None
 
 
 def _say(msg):

@@ -285,6 +285,139 @@ Tensors norm_rope_backward(const at::Tensor& g, const at::Tensor& h, const OptTe
   return {b.dx, b.dweight};
 }
 
+// ---- The MX cache (velograd_amd/kernels/mx_cache.py) ----
+
+// A dense tensor with data of its own on the current device, of any strides.
+bool dense(const at::Tensor& t) {
+  return t.is_cuda() && t.has_storage() && !t.is_neg() &&
+         !t.unsafeGetTensorImpl()->is_python_dispatch() && t.layout() == at::kStrided &&
+         t.get_device() == c10::hip::current_device();
+}
+
+struct MxShape {
+  int64_t pages = 0, kv_heads = 0, page_size = 0, head_dim = 0;
+  int32_t format = -1;  // -1: the tensors are no cache that the fast path takes
+};
+
+MxShape mx_shape(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc,
+                 const at::Tensor& vs) {
+  MxShape s;
+  const bool fp4 = kc.scalar_type() == at::kFloat4_e2m1fn_x2;
+  if ((!fp4 && kc.scalar_type() != at::kFloat8_e4m3fn) || vc.scalar_type() != kc.scalar_type() ||
+      ks.scalar_type() != at::kFloat8_e8m0fnu || vs.scalar_type() != at::kFloat8_e8m0fnu ||
+      kc.dim() != 4 || ks.dim() != 4 || vc.sizes() != kc.sizes() || vs.sizes() != ks.sizes())
+    return s;
+  for (const at::Tensor* t : {&kc, &ks, &vc, &vs})
+    if (!dense(*t) || !t->is_contiguous()) return s;
+  s.pages = kc.size(0);
+  s.kv_heads = kc.size(1);
+  s.page_size = kc.size(2);
+  s.head_dim = kc.size(3) * (fp4 ? 2 : 1);
+  if (ks.size(0) != s.pages || ks.size(1) != s.kv_heads || ks.size(2) * 32 != s.head_dim ||
+      ks.size(3) != s.page_size || s.pages == 0)
+    return s;
+  s.format = fp4 ? VELOGRAD_MX_E2M1 : VELOGRAD_MX_E4M3;
+  return s;
+}
+
+// [tokens, heads, head_dim] rows with unit stride along head_dim.
+bool mx_rows(const at::Tensor& t, const MxShape& s, at::ScalarType type) {
+  return t.dim() == 3 && t.scalar_type() == type && t.size(2) == s.head_dim && t.stride(2) == 1 &&
+         dense(t);
+}
+
+bool mx_index(const at::Tensor& t, at::ScalarType type, int64_t n) {
+  return t.dim() == 1 && t.scalar_type() == type && t.size(0) == n && dense(t) && t.is_contiguous();
+}
+
+// [q_out (undefined without q)].
+Tensors mx_write(const OptTensor& q, const at::Tensor& k, const at::Tensor& v,
+                 const OptTensor& cos_sin, const OptTensor& positions, const at::Tensor& kc,
+                 const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs,
+                 const at::Tensor& slots) {
+  const int32_t code = dtype_code(k.scalar_type());
+  const MxShape s = mx_shape(kc, ks, vc, vs);
+  if (code < 0 || s.format < 0 || !mx_rows(k, s, k.scalar_type()) || !mx_rows(v, s, k.scalar_type()))
+    return {};
+  const int64_t tokens = k.size(0);
+  if (tokens == 0 || v.size(0) != tokens || k.size(1) != s.kv_heads || v.size(1) != s.kv_heads ||
+      !mx_index(slots, at::kLong, tokens))
+    return {};
+  const bool rope = positions.has_value();
+  if (rope && (!cos_sin.has_value() || !mx_index(*positions, at::kLong, tokens) || cos_sin->dim() != 2 ||
+               cos_sin->scalar_type() != at::kFloat || cos_sin->size(1) != s.head_dim ||
+               !dense(*cos_sin) || !cos_sin->is_contiguous()))
+    return {};
+  at::Tensor q_out;
+  if (q.has_value()) {
+    if (!rope || !mx_rows(*q, s, k.scalar_type()) || q->size(0) != tokens || q->size(1) == 0) return {};
+    q_out = at::empty(q->sizes(), q->options());
+  }
+  const bool has_q = q_out.defined();
+  check(velograd_mx_cache_write(
+            has_q ? q->data_ptr() : nullptr, k.data_ptr(), v.data_ptr(),
+            has_q ? q_out.data_ptr() : nullptr, rope ? cos_sin->data_ptr<float>() : nullptr,
+            rope ? positions->data_ptr<int64_t>() : nullptr, slots.data_ptr<int64_t>(),
+            kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), tokens,
+            has_q ? q->size(1) : 0, s.kv_heads, s.head_dim, has_q ? q->stride(0) : 0,
+            has_q ? q->stride(1) : 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            rope ? cos_sin->size(0) : 0, s.pages, s.page_size, code, s.format, stream_of(k)),
+        "velograd_mx_cache_write");
+  return {q_out};
+}
+
+// [k, v] in the dtype of VELOGRAD_DTYPE code `dtype`.
+Tensors mx_read(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc,
+                const at::Tensor& vs, const at::Tensor& slots, int64_t dtype) {
+  const MxShape s = mx_shape(kc, ks, vc, vs);
+  if (s.format < 0 || slots.dim() != 1 || slots.size(0) == 0 ||
+      !mx_index(slots, at::kLong, slots.size(0)))
+    return {};
+  const auto type = dtype == VELOGRAD_DTYPE_F32 ? at::kFloat : dtype == VELOGRAD_DTYPE_F16 ? at::kHalf : at::kBFloat16;
+  const auto options = kc.options().dtype(type);
+  at::Tensor k = at::empty({slots.size(0), s.kv_heads, s.head_dim}, options);
+  at::Tensor v = at::empty({slots.size(0), s.kv_heads, s.head_dim}, options);
+  check(velograd_mx_cache_read(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+                               slots.data_ptr<int64_t>(), k.data_ptr(), v.data_ptr(), slots.size(0),
+                               s.kv_heads, s.head_dim, s.pages, s.page_size, (int32_t)dtype, s.format,
+                               stream_of(kc)),
+        "velograd_mx_cache_read");
+  return {k, v};
+}
+
+// [out, lse (undefined unless asked for)].
+Tensors mx_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& ks,
+                     const at::Tensor& vc, const at::Tensor& vs, const at::Tensor& table,
+                     const at::Tensor& lengths, const OptTensor& starts, double scale, bool causal,
+                     bool want_lse) {
+  const int32_t code = dtype_code(q.scalar_type());
+  const MxShape s = mx_shape(kc, ks, vc, vs);
+  if (code < 0 || s.format < 0 || !mx_rows(q, s, q.scalar_type())) return {};
+  const int64_t tokens = q.size(0), heads = q.size(1);
+  if (tokens == 0 || heads == 0 || heads % s.kv_heads != 0 || table.dim() != 2 ||
+      table.scalar_type() != at::kInt || !dense(table) || table.size(0) == 0 || table.size(1) == 0 ||
+      table.stride(1) != 1 || !mx_index(lengths, at::kInt, table.size(0)))
+    return {};
+  const int64_t sequences = table.size(0);
+  if (starts.has_value() ? !mx_index(*starts, at::kInt, sequences + 1) : tokens != sequences) return {};
+  const size_t bytes = velograd_mx_cache_attention_workspace_bytes(
+      tokens, sequences, heads, s.kv_heads, s.head_dim, table.size(1), s.page_size,
+      starts.has_value() ? 1 : 0, q.get_device());
+  at::Tensor out = at::empty(q.sizes(), q.options()), lse, ws;
+  if (want_lse) lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
+  if (bytes != 0) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check(velograd_mx_cache_attention(
+            q.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+            table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(),
+            starts.has_value() ? starts->data_ptr<int32_t>() : nullptr, out.data_ptr(),
+            want_lse ? lse.data_ptr<float>() : nullptr, bytes != 0 ? ws.data_ptr() : nullptr, bytes,
+            tokens, sequences, heads, s.kv_heads, s.head_dim, q.stride(0), q.stride(1),
+            table.stride(0), table.size(1), s.pages, s.page_size, (float)scale, causal ? 1 : 0, code,
+            s.format, stream_of(q)),
+        "velograd_mx_cache_attention");
+  return {out, lse};
+}
+
 // The interpreter lock given up for a scope (pybind11's own guard looks its internals up as well, a
 // tenth of a microsecond a call).
 struct Unlocked {
@@ -322,4 +455,15 @@ PYBIND11_MODULE(_fastpath, m) {
   m.def("norm_rope_backward", &norm_rope_backward, NoGil(), pybind11::arg("grad_y"),
         pybind11::arg("h"), pybind11::arg("weight"), pybind11::arg("inv_rms"),
         pybind11::arg("base"));
+  m.def("mx_write", &mx_write, NoGil(), pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"),
+        pybind11::arg("cos_sin"), pybind11::arg("positions"), pybind11::arg("k_codes"),
+        pybind11::arg("k_scales"), pybind11::arg("v_codes"), pybind11::arg("v_scales"),
+        pybind11::arg("slots"));
+  m.def("mx_read", &mx_read, NoGil(), pybind11::arg("k_codes"), pybind11::arg("k_scales"),
+        pybind11::arg("v_codes"), pybind11::arg("v_scales"), pybind11::arg("slots"),
+        pybind11::arg("dtype"));
+  m.def("mx_attention", &mx_attention, NoGil(), pybind11::arg("q"), pybind11::arg("k_codes"),
+        pybind11::arg("k_scales"), pybind11::arg("v_codes"), pybind11::arg("v_scales"),
+        pybind11::arg("block_table"), pybind11::arg("lengths"), pybind11::arg("q_starts"),
+        pybind11::arg("scale"), pybind11::arg("causal"), pybind11::arg("lse"));
 }

@@ -160,7 +160,21 @@ def _stream(device: torch.device) -> int:
     return current(device)
 
 
+def _fast(cache, *given):
+    """The C++ fast path, where the arguments are tensors; it returns nothing for a call that it leaves to
+    the general path below."""
+    if isinstance(cache, tuple) and len(cache) == 4 and all(isinstance(t, torch.Tensor) for t in cache) \
+            and all(isinstance(t, torch.Tensor) for t in given):
+        return _lib.fastpath()
+    return None
+
+
 def _write(q, k, v, cos_sin, positions, cache, slots):
+    fp = _fast(cache, k, v, slots, *(t for t in (q, cos_sin, positions) if t is not None))
+    if fp is not None:
+        done = fp.mx_write(q, k, v, cos_sin, positions, *cache, slots)
+        if done:
+            return done[0]
     shape, device = _check_cache(cache)
     code = _check_rows(k, "k", device, shape.kv_heads, shape.head_dim)
     _check_rows(v, "v", device, shape.kv_heads, shape.head_dim)
@@ -241,6 +255,11 @@ def mx_cache_read(cache: MXCache, slots: torch.Tensor,
     """The keys and values that the slots (int64 [tokens], any order) hold: (k, v), each
     [tokens, kv_heads, head_dim] in `dtype`.  Exact in float32 and bfloat16; float16 rounds, and overflows
     to infinity past its range.  A slot outside the cache reads as zeros."""
+    fp = _fast(cache, slots)
+    if fp is not None and dtype in _lib.TORCH_DTYPE_CODES:
+        done = fp.mx_read(*cache, slots, _lib.TORCH_DTYPE_CODES[dtype])
+        if done:
+            return done[0], done[1]
     shape, device = _check_cache(cache)
     _check_tensor(slots, "slots", device, torch.int64, 1)
     if dtype not in _lib.TORCH_DTYPE_CODES:
@@ -279,6 +298,13 @@ def mx_cache_attention(q: torch.Tensor, cache: MXCache, block_table: torch.Tenso
     no key, and a row of q past the last sequence, gives 0 and -inf.  Keys on a page outside the cache are
     not seen.
     """
+    fp = _fast(cache, q, block_table, lengths, *(() if q_starts is None else (q_starts,)))
+    if fp is not None and q.dim() == 3:
+        done = fp.mx_attention(q, *cache, block_table, lengths, q_starts,
+                               1.0 / math.sqrt(max(1, q.shape[2])) if scale is None else float(scale),
+                               bool(causal), bool(return_lse))
+        if done:
+            return (done[0], done[1]) if return_lse else done[0]
     shape, device = _check_cache(cache)
     code = _check_rows(q, "q", device, None, shape.head_dim)
     tokens, heads = q.shape[0], q.shape[1]
