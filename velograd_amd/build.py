@@ -11,6 +11,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -51,6 +53,10 @@ HIPCC_FLAGS = [
     "-Wall",
 ]
 
+# Of single sources.  The attention's accumulators stay in the vector registers that its softmax rescales
+# (the compiler's default moves each to and from the accumulation registers in every step).
+FILE_FLAGS = {"mx_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 
 def find_hipcc() -> str:
     for cand in (os.environ.get("HIPCC"), shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
@@ -59,9 +65,7 @@ def find_hipcc() -> str:
     raise RuntimeError("hipcc not found: the HIP toolchain (ROCm) is required to build")
 
 
-def _hipcc(srcs, out: str, verbose: bool) -> None:
-    tmp = out + ".tmp"
-    cmd = [find_hipcc(), *HIPCC_FLAGS, "-I", INCLUDE_DIR, "-I", CSRC_DIR, *srcs, "-o", tmp]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -69,6 +73,21 @@ def _hipcc(srcs, out: str, verbose: bool) -> None:
         raise RuntimeError(
             "hipcc failed (exit %d):\n%s\n%s" % (proc.returncode, proc.stdout, proc.stderr)
         )
+
+
+def _hipcc(srcs, out: str, verbose: bool) -> None:
+    """Compile the sources side by side, then link them into `out`."""
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    tmp = out + ".tmp"
+    with tempfile.TemporaryDirectory() as d:
+        objects = [os.path.join(d, os.path.basename(src) + ".o") for src in srcs]
+        with ThreadPoolExecutor(max_workers=len(srcs)) as pool:
+            jobs = [pool.submit(_run, [find_hipcc(), *flags, *FILE_FLAGS.get(os.path.basename(src), []),
+                                       "-I", INCLUDE_DIR, "-I", CSRC_DIR, "-c", src, "-o", obj], verbose)
+                    for src, obj in zip(srcs, objects)]
+            for job in jobs:
+                job.result()
+        _run([find_hipcc(), f"--offload-arch={OFFLOAD_ARCH}", "-shared", "-fPIC", *objects, "-o", tmp], verbose)
     os.replace(tmp, out)
 
 

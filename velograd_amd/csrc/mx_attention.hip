@@ -32,6 +32,10 @@ using namespace vg;
 constexpr int kTile = 32;   // keys of one step
 constexpr int kWaves = 4;   // waves of a workgroup
 constexpr int kRows = 16;   // query rows of a wave
+#ifndef VG_STEP_GROUPS
+#define VG_STEP_GROUPS 8
+#endif
+constexpr int kStepGroups = VG_STEP_GROUPS;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -52,7 +56,7 @@ struct AttnArgs {
   int32_t width;           // pages of a row of the table
   int32_t pages, page_shift;
   int32_t causal;
-  int32_t row_tiles;
+  int32_t row_tiles, tile_rows;
   int32_t chunk, splits;   // keys of a split (a multiple of kTile), splits of the longest sequence
   float scale_log2;        // scale * log2(e)
 };
@@ -171,6 +175,23 @@ __device__ __forceinline__ void split_parts(float* f, u32x4* out) {
         const float a = __builtin_bit_cast(float, w << 16), b = __builtin_bit_cast(float, w & 0xffff0000u);
         f[2 * i] = __builtin_isfinite(a) ? f[2 * i] - a : 0.0f;
         f[2 * i + 1] = __builtin_isfinite(b) ? f[2 * i + 1] - b : 0.0f;
+      }
+    }
+  }
+}
+
+// The same for probabilities (in [0, 2^8], or NaN): no infinities to look for.
+template <int PARTS>
+__device__ __forceinline__ void split_probs(float* f, u32x4* out) {
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = pack_bf16(f[2 * i], f[2 * i + 1]);
+      out[p][i] = w;
+      if (p + 1 < PARTS) {
+        f[2 * i] -= __builtin_bit_cast(float, w << 16);
+        f[2 * i + 1] -= __builtin_bit_cast(float, w & 0xffff0000u);
       }
     }
   }
@@ -465,9 +486,432 @@ __global__ __launch_bounds__(kWaves * 64) void mx_attention_kernel(const AttnArg
     a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(l)) * 0.693147180559945309f;
 }
 
-// Joins the splits of one (token, head) row; rows of tiles that had one split are left alone.
-template <int DT>
-__global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a, int32_t dim) {
+// ------------------------------------------------------------------------------------------
+// Few rows a sequence: single and drafted tokens.
+// ------------------------------------------------------------------------------------------
+// A workgroup's four waves take the same 16 NQ query rows, each a quarter of the split's keys in one run,
+// and add up at the end through LDS.  A wave reads its keys' codes straight into registers, one step of 32
+// ahead of the products.  Page numbers come from one load of a lane each for 64 groups of 8 keys (512
+// keys), and reach the addresses as scalars: a step's two halves of 16 keys lie on one page each.
+constexpr int kRunGroups = 64;
+constexpr int kRunKeys = 8 * kRunGroups;
+
+template <int D, int FMT>
+struct KeyTile {
+  using S = Shape<D, FMT, VELOGRAD_DTYPE_BF16>;
+  static constexpr int kWordsK = S::kKBytes / 4;
+  static constexpr int kWordsV = S::kVBytes < 4 ? 1 : S::kVBytes / 4;
+  uint32_t kw[2][kWordsK];
+  uint32_t ks[2][S::kKScales];
+  uint32_t vw[8][kWordsV];
+  u32x2 vs;
+};
+
+struct CacheView {
+  const uint8_t *kc, *ks, *vc, *vs;  // of the head
+  int64_t code_page, scale_page;     // bytes of a page, all heads
+  int32_t page_shift;
+};
+
+// Keys t .. t + 31, whose halves lie on pages p0 and p1 (places a0 and a1 of them).
+template <int D, int FMT>
+__device__ __forceinline__ void load_tile(const CacheView& c, int32_t p0, int32_t a0, int32_t p1, int32_t a1,
+                                          int32_t n, int32_t g, KeyTile<D, FMT>& t) {
+  using S = typename KeyTile<D, FMT>::S;
+  const int64_t c0 = p0 * c.code_page + (int64_t)a0 * S::kRowBytes, c1 = p1 * c.code_page + (int64_t)a1 * S::kRowBytes;
+  const int64_t s0 = p0 * c.scale_page + a0, s1 = p1 * c.scale_page + a1;
+  const int32_t gk = n >> 2;  // the lane's group of 8 keys, as a row of K
+  const uint8_t* kp = c.kc + (gk & 2 ? c1 : c0) + (8 * (gk & 1) + (n & 3)) * S::kRowBytes + g * S::kKBytes;
+  const uint8_t* kq = c.ks + (gk & 2 ? s1 : s0) + (((g * (D / 4)) / 32) << c.page_shift) + 8 * (gk & 1) + (n & 3);
+  const uint8_t* vp = c.vc + (g & 2 ? c1 : c0) + 8 * (g & 1) * S::kRowBytes + n * S::kVBytes;
+  const uint8_t* vq = c.vs + (g & 2 ? s1 : s0) + (((n * (D / 16)) / 32) << c.page_shift) + 8 * (g & 1);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    load_words<S::kKBytes>(kp + 4 * u * S::kRowBytes, t.kw[u]);
+#pragma unroll
+    for (int b = 0; b < S::kKScales; ++b) t.ks[u][b] = kq[((int64_t)b << c.page_shift) + 4 * u];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load_words<S::kVBytes>(vp + i * S::kRowBytes, t.vw[i]);
+  t.vs = *reinterpret_cast<const u32x2*>(vq);
+}
+
+// S^T of the tile for one query tile: x[i] is the score of key 8 g + i, unscaled.
+template <int D, int FMT, int PARTS>
+__device__ __forceinline__ void decode_keys(const KeyTile<D, FMT>& t, u32x4 (*kf)[D / 32]) {
+  using S = typename KeyTile<D, FMT>::S;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float scale[S::kKScales];
+#pragma unroll
+    for (int b = 0; b < S::kKScales; ++b) scale[b] = scale_arg(t.ks[u][b]);
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int pair = 4 * s + i;  // of the lane's D/8 pairs
+        kf[u][s][i] = decode_pair<FMT>(t.kw[u][pair / S::kPerWord], scale[pair / 16 % S::kKScales], pair % S::kPerWord);
+      }
+  }
+}
+
+// V^T of the tile: fragment j is dim n D/16 + j of keys 8 g .. 8 g + 7.
+template <int D, int FMT>
+__device__ __forceinline__ void decode_values(const KeyTile<D, FMT>& t, u32x4* vf) {
+  using S = typename KeyTile<D, FMT>::S;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // The conversion reads its scale's exponent alone, so the bits around the byte may be anything.
+    const uint32_t w = t.vs[i >> 1];
+    const float s0 = __builtin_bit_cast(float, i & 1 ? w << 7 : w << 23);
+    const float s1 = __builtin_bit_cast(float, i & 1 ? w >> 1 : w << 15);
+#pragma unroll
+    for (int d = 0; d < S::kOut / 2; ++d) {
+      const uint32_t u0 = decode_pair<FMT>(t.vw[2 * i][d / S::kPerWord], s0, d % S::kPerWord);
+      const uint32_t u1 = decode_pair<FMT>(t.vw[2 * i + 1][d / S::kPerWord], s1, d % S::kPerWord);
+      vf[2 * d][i] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
+      vf[2 * d + 1][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+    }
+  }
+}
+
+// One query tile's running state: rows in lanes (column n), keys or dims in registers.
+template <int D>
+struct RowState {
+  f32x4 acc[D / 16];
+  float m, l;
+};
+
+// x becomes the probabilities' exponents' arguments less the maximum; updates m, l, acc.
+template <int D>
+__device__ __forceinline__ void softmax_step(float* x, RowState<D>& r) {
+  float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
+                              __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
+  // The running maximum moves only when a row's new maximum passes it by 8 (p stays below 2^8, which
+  // costs fp32 nothing): most steps rescale nothing.
+  if (__ballot(top > r.m + 8.0f) != 0) {
+    top = across_g(top, false);
+    const float next = top > r.m + 8.0f ? top : r.m;  // for each row by itself
+    const float f = __builtin_amdgcn_exp2f(r.m - next);
+    r.m = next;
+    r.l *= f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) r.acc[j] *= f;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - r.m);
+  r.l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+}
+
+// Bytes of w that are 0xFF (scales: a block marked NaN), or 0x7F with any sign (e4m3's NaN): bit 7 of each.
+__device__ __forceinline__ uint32_t nan_scales(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <int D, int FMT>
+__device__ __forceinline__ bool any_nan(const KeyTile<D, FMT>& t) {
+  uint32_t any = nan_scales(t.vs[0]) | nan_scales(t.vs[1]);
+  if constexpr (FMT == VELOGRAD_MX_E4M3)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w) any |= nan_codes(t.vw[i][w]);
+  return __ballot(any != 0) != 0;
+}
+
+// A NaN among the values of a key that only some of the rows see would reach the others as 0 * NaN: its
+// codes are taken out of the tile, and the rows that do see it get NaN by a product of flags.
+template <int D, int FMT, int NQ>
+__device__ __forceinline__ void keep_nan_apart(KeyTile<D, FMT>& t, const float (*x)[8], RowState<D>* rows) {
+  constexpr int kOut = D / 16;
+  constexpr int kEach = FMT == VELOGRAD_MX_E4M3 ? kOut : 1;  // e2m1 has no NaN of its own: blocks only
+  u32x4 seen[NQ], blocks;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = t.vs[i >> 1] >> (16 * (i & 1));
+    blocks[i] = ((w & 0xffu) == 0xffu ? 0x3f80u : 0u) | ((w & 0xff00u) == 0xff00u ? 0x3f800000u : 0u);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+      seen[q][i] = (x[q][2 * i] != -__builtin_inff() ? 0x3f80u : 0u) |
+                   (x[q][2 * i + 1] != -__builtin_inff() ? 0x3f800000u : 0u);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    u32x4 f = blocks;
+    if constexpr (FMT == VELOGRAD_MX_E4M3) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w0 = nan_codes(t.vw[2 * i][e >> 2]) >> (8 * (e & 3) + 7);
+        const uint32_t w1 = nan_codes(t.vw[2 * i + 1][e >> 2]) >> (8 * (e & 3) + 7);
+        f[i] |= (w0 & 1u) * 0x3f80u | (w1 & 1u) * 0x3f800000u;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const f32x4 hit = mfma(f, seen[q], f32x4{0, 0, 0, 0});
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kOut; ++j)
+          if (kEach == 1 || j == e) rows[q].acc[j][i] = hit[i] > 0.0f ? __builtin_nanf("") : rows[q].acc[j][i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool block = ((t.vs[i >> 2] >> (8 * (i & 3))) & 0xffu) == 0xffu;
+#pragma unroll
+    for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w) {
+      if constexpr (FMT == VELOGRAD_MX_E4M3) t.vw[i][w] &= ~((nan_codes(t.vw[i][w]) >> 7) * 0xffu);
+      if (block) t.vw[i][w] = 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) t.vs[i] &= ~(nan_scales(t.vs[i]));  // 0xFF -> 0x7F
+}
+
+// A row's result, unnormalised sums to the workspace where the keys are split, else out and lse.
+template <int D, int DT>
+__device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& r, int64_t orow, int32_t split,
+                                          bool partial, int32_t g) {
+  constexpr int kOut = D / 16;
+  if (partial) {
+    float* po = a.part_o + (orow * a.splits + split) * D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < kOut; j += 4)
+        *reinterpret_cast<f32x4*>(po + (4 * g + i) * kOut + j) =
+            f32x4{r.acc[j][i], r.acc[j + 1][i], r.acc[j + 2][i], r.acc[j + 3][i]};
+    if (g == 0) {
+      a.part_ml[(orow * a.splits + split) * 2] = r.m;
+      a.part_ml[(orow * a.splits + split) * 2 + 1] = r.l;
+    }
+    return;
+  }
+  const bool empty = r.l == 0.0f;
+  const float inv = empty ? 0.0f : 1.0f / r.l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[kOut];
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) f[j] = empty ? 0.0f : r.acc[j][i] * inv;
+    const int64_t e = orow * D + (4 * g + i) * kOut;
+    if constexpr (kOut >= Codec<DT>::kVec) {
+#pragma unroll
+      for (int j = 0; j < kOut; j += Codec<DT>::kVec) store16<DT>(a.out, e + j, Codec<DT>::pack(f + j));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kOut; ++j) Codec<DT>::store1(a.out, e + j, f[j]);
+    }
+  }
+  if (a.lse != nullptr && g == 0)
+    a.lse[orow] = empty ? -__builtin_inff() : (r.m + log2f(r.l)) * 0.693147180559945309f;
+}
+
+// A query row's fragments: dims g D/4 + 8 s .. + 7 for product s; zeros for a row that is none.
+template <int D, int DT>
+__device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, bool ok,
+                                           u32x4 (*qf)[Shape<D, VELOGRAD_MX_E2M1, DT>::kQParts]) {
+  using S = Shape<D, VELOGRAD_MX_E2M1, DT>;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (ok) {
+      Codec<DT>::unpack(load16_any<DT>(a.q, e + 8 * s), f);
+      if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, e + 8 * s + 4), f + 4);
+    }
+    split_parts<S::kQParts>(f, qf[s]);
+  }
+}
+
+// Waves of a SIMD that the registers are held to: as many as take no spills.
+constexpr int step_occupancy(int dim, int fmt, int dtype) {
+  const bool small = fmt == VELOGRAD_MX_E2M1, plain = dtype == VELOGRAD_DTYPE_BF16;
+  return dim == 64 ? (small || plain ? 4 : 3) : dim == 128 ? (small && plain ? 3 : 2) : 1;
+}
+
+template <int D, int FMT, int DT, int NQ>
+__global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT)) void mx_attention_step_kernel(const AttnArgs a) {
+  using S = Shape<D, FMT, DT>;
+  constexpr int kTileRows = kRows * NQ;
+  // Heads fastest, then row tiles, then splits.
+  const uint32_t tile_split = blockIdx.x / (uint32_t)a.kv_heads;
+  const int32_t h = (int32_t)(blockIdx.x - tile_split * (uint32_t)a.kv_heads);
+  const int32_t split = (int32_t)(tile_split / (uint32_t)a.row_tiles);
+  const RowTile r = find_tile(a, (int32_t)(tile_split - (uint32_t)split * (uint32_t)a.row_tiles), kTileRows);
+  if (r.row0 < 0 || r.row0 >= r.rows) return;
+  const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
+  const int32_t most = row_limit(a, r, last / a.group);      // keys that the tile's last row sees,
+  const int32_t clear = row_limit(a, r, r.row0 / a.group);   // and that all its rows see
+  const int32_t active = splits_of(a, most);
+  if (split >= active) return;
+  const int32_t wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+
+  // The wave's keys: a quarter of the split's steps.
+  const int32_t from = split * a.chunk;
+  const int32_t till = from + a.chunk < most ? from + a.chunk : most;
+  const int32_t steps = (till - from + kTile - 1) / kTile;
+  const int32_t begin = from + (steps * wave / kWaves) * kTile;
+  int32_t end = from + (steps * (wave + 1) / kWaves) * kTile;
+  if (end > till) end = till;
+
+  bool row_ok[NQ];
+  int32_t limit[NQ];
+  int64_t orow[NQ];
+  u32x4 qf[NQ][S::kSteps][S::kQParts];
+  RowState<D> rows[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int32_t row = r.row0 + kRows * q + n;
+    row_ok[q] = row < r.rows;
+    const int32_t fresh = row_ok[q] ? row / a.group : 0;
+    const int32_t head = h * a.group + (row_ok[q] ? row - fresh * a.group : 0);
+    limit[q] = row_ok[q] ? row_limit(a, r, fresh) : 0;
+    const int64_t tok = r.tok0 + fresh;
+    orow[q] = tok * a.q_heads + head;
+    load_query<D, DT>(a, tok * a.q_t + head * a.q_h + g * (D / 4), row_ok[q], qf[q]);
+#pragma unroll
+    for (int j = 0; j < S::kOut; ++j) rows[q].acc[j] = f32x4{0, 0, 0, 0};
+    rows[q].m = -3.0e38f;
+    rows[q].l = 0.0f;
+  }
+
+  const int32_t* table = a.table + (int64_t)(r.seq < 0 ? 0 : r.seq) * a.table_stride;
+  const int32_t page_mask = (1 << a.page_shift) - 1;
+  CacheView c;
+  c.page_shift = a.page_shift;
+  c.code_page = (int64_t)a.kv_heads * S::kRowBytes << a.page_shift;
+  c.scale_page = (int64_t)a.kv_heads * (D / 32) << a.page_shift;
+  c.kc = a.kc + ((int64_t)h * S::kRowBytes << a.page_shift);
+  c.vc = a.vc + ((int64_t)h * S::kRowBytes << a.page_shift);
+  c.ks = a.ks + ((int64_t)h * (D / 32) << a.page_shift);
+  c.vs = a.vs + ((int64_t)h * (D / 32) << a.page_shift);
+
+  for (int32_t run = begin; run < end; run += kRunKeys) {
+    const int32_t run_end = run + kRunKeys < end ? run + kRunKeys : end;
+    int32_t at = (run + 8 * lane) >> a.page_shift;
+    if (at >= a.width) at = a.width - 1;
+    int32_t page = table[at];
+    const bool none = (uint32_t)page >= (uint32_t)a.pages;
+    if (none) page = 0;
+    const uint64_t missing = __ballot(none);
+
+    auto fetch = [&](int32_t t0, KeyTile<D, FMT>& t) {
+      const int32_t i = (t0 - run) >> 3;
+      const int32_t p0 = __builtin_amdgcn_readlane(page, i), p1 = __builtin_amdgcn_readlane(page, i + 2);
+      load_tile<D, FMT>(c, p0, t0 & page_mask, p1, (t0 + 16) & page_mask, n, g, t);
+    };
+    auto use = [&](int32_t t0, KeyTile<D, FMT>& t) {
+      float x[NQ][8];
+      {
+        u32x4 kf[2][S::kSteps];
+        decode_keys<D, FMT, S::kQParts>(t, kf);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            f32x4 sc = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+              for (int p = S::kQParts - 1; p >= 0; --p) sc = mfma(kf[u][s], qf[q][s][p], sc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[q][4 * u + i] = sc[i] * a.scale_log2;
+          }
+      }
+      const uint32_t gone = (uint32_t)(missing >> ((t0 - run) >> 3)) & 0xfu;
+      const bool masked = t0 + kTile > clear || gone != 0;
+      if (masked) {
+        const bool bad = (gone >> g) & 1u;
+        // Of the lane's 8 keys: how many there are, and how many the row sees.
+        const int32_t here = bad ? 0 : r.length - t0 - 8 * g;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const int32_t see = bad ? 0 : limit[q] - t0 - 8 * g;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[q][i] = i < see ? x[q][i] : -__builtin_inff();
+        }
+        // What lies behind the sequence's end may be anything: it is taken as zeros.
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w) t.vw[i][w] = i < here ? t.vw[i][w] : 0;
+          const uint32_t m = 0xffu << (8 * (i & 3));
+          t.vs[i >> 2] = i < here ? t.vs[i >> 2] : (t.vs[i >> 2] & ~m) | (0x7f7f7f7fu & m);
+        }
+      }
+      if (masked && clear < most && any_nan<D, FMT>(t)) keep_nan_apart<D, FMT, NQ>(t, x, rows);
+      u32x4 vf[S::kOut];
+      decode_values<D, FMT>(t, vf);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        softmax_step<D>(x[q], rows[q]);
+        u32x4 pf[S::kPParts];
+        split_probs<S::kPParts>(x[q], pf);
+#pragma unroll
+        for (int p = S::kPParts - 1; p >= 0; --p)
+#pragma unroll
+          for (int j = 0; j < S::kOut; ++j) rows[q].acc[j] = mfma(vf[j], pf[p], rows[q].acc[j]);
+      }
+    };
+    // Each step's loads are issued a step before, without a branch around them (past the run's end the last
+    // step's again): the wait for one step's codes then leaves the next one's in flight.
+    const int32_t final = run + (run_end - 1 - run) / kTile * kTile;
+    KeyTile<D, FMT> t0, t1;
+    fetch(run, t0);
+    for (int32_t t = run;; t += 2 * kTile) {
+      fetch(t + kTile < final ? t + kTile : final, t1);
+      use(t, t0);
+      if (t >= final) break;
+      fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
+      use(t + kTile, t1);
+      if (t + kTile >= final) break;
+    }
+  }
+
+  // Waves 2, 3 hand their sums to 0, 1, then 1 to 0, in the accumulators' own layout.
+  __shared__ float buf[kWaves / 2][D / 4 + 2][64];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+    for (int w = kWaves / 2; w >= 1; w >>= 1) {
+      if (wave >= w && wave < 2 * w) {
+#pragma unroll
+        for (int j = 0; j < S::kOut; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) buf[wave - w][4 * j + i][lane] = rows[q].acc[j][i];
+        buf[wave - w][D / 4][lane] = rows[q].m;
+        buf[wave - w][D / 4 + 1][lane] = rows[q].l;
+      }
+      __syncthreads();
+      if (wave < w) {
+        const float mo = buf[wave][D / 4][lane];
+        const float next = __builtin_fmaxf(rows[q].m, mo);
+        const float f = __builtin_amdgcn_exp2f(rows[q].m - next), fo = __builtin_amdgcn_exp2f(mo - next);
+        rows[q].m = next;
+        rows[q].l = rows[q].l * f + buf[wave][D / 4 + 1][lane] * fo;
+#pragma unroll
+        for (int j = 0; j < S::kOut; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            rows[q].acc[j][i] = rows[q].acc[j][i] * f + buf[wave][4 * j + i][lane] * fo;
+      }
+      __syncthreads();
+    }
+  }
+  if (wave != 0) return;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    rows[q].l = across_g(rows[q].l, true);
+    if (row_ok[q]) store_row<D, DT>(a, rows[q], orow[q], split, active > 1, g);
+  }
+}
+
+// Joins the splits of one (token, head) row; rows of tiles that had one split are left alone.  D/4 lanes
+// hold the row, the workgroup's other lanes take other splits, and LDS adds them up.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a) {
+  constexpr int kLanes = D / 4, kSets = 256 / kLanes;
   const int64_t orow = blockIdx.x;
   const int32_t tok = (int32_t)(orow / a.q_heads), head = (int32_t)(orow - (int64_t)tok * a.q_heads);
   RowTile r;
@@ -483,44 +927,69 @@ __global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a
   r.rows = r.fresh * a.group;
   r.length = held_tokens(a, r.seq);
   const int32_t row = (tok - r.tok0) * a.group + head % a.group;
-  int32_t last = row - row % (kWaves * kRows) + kWaves * kRows;
+  int32_t last = row - row % a.tile_rows + a.tile_rows;
   if (last > r.rows) last = r.rows;
   const int32_t active = splits_of(a, row_limit(a, r, (last - 1) / a.group));
   if (active <= 1) return;
+
   const float* ml = a.part_ml + orow * a.splits * 2;
-  const float* po = a.part_o + orow * a.splits * dim;
+  const int32_t d = threadIdx.x % kLanes, set = threadIdx.x / kLanes;
+  const float* po = a.part_o + orow * a.splits * D + 4 * d;
   float m = -3.0e38f;
-  for (int32_t s = 0; s < active; ++s) m = __builtin_fmaxf(m, ml[2 * s]);
-  float l = 0.0f, o = 0.0f;
-  const int32_t d = threadIdx.x;
-  for (int32_t s = 0; s < active; ++s) {
+  for (int32_t s = threadIdx.x & 63; s < active; s += 64) m = __builtin_fmaxf(m, ml[2 * s]);
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, w));
+  float l = 0.0f;
+  f32x4 o = {0, 0, 0, 0};
+  for (int32_t s = set; s < active; s += kSets) {
     const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
     l += ml[2 * s + 1] * f;
-    if (d < dim) o += po[(int64_t)s * dim + d] * f;
+    o += *reinterpret_cast<const f32x4*>(po + (int64_t)s * D) * f;
   }
-  const bool empty = l == 0.0f;
-  if (d < dim) Codec<DT>::store1(a.out, orow * dim + d, empty ? 0.0f : o / l);
-  if (a.lse != nullptr && d == 0)
-    a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(l)) * 0.693147180559945309f;
+  __shared__ float sums[kSets][D + 4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sums[set][4 * d + i] = o[i];
+  if (d == 0) sums[set][D] = l;
+  __syncthreads();
+  const int32_t e = threadIdx.x;
+  if (e >= D) return;
+  float total = 0.0f, x = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kSets; ++i) {
+    total += sums[i][D];
+    x += sums[i][e];
+  }
+  const bool empty = total == 0.0f;
+  Codec<DT>::store1(a.out, orow * D + e, empty ? 0.0f : x / total);
+  if (a.lse != nullptr && e == 0)
+    a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(total)) * 0.693147180559945309f;
 }
 
 // How a call is laid out: workgroups over row tiles, heads and splits of the keys.
 struct AttnPlan {
   int64_t row_tiles;
+  int32_t tile_rows;
+  int32_t query_tiles;  // of 16 rows a wave, in the kernel for few rows; 0: the kernel for many
   int32_t chunk, splits;
 };
 
 AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, bool ragged,
                         int64_t most, int cus) {
   AttnPlan p;
-  const int64_t group = q_heads / kv_heads, tile = kWaves * kRows;
-  p.row_tiles = ragged ? q_tokens * group / tile + batch + 2 : batch * ((group + tile - 1) / tile);
-  // Splits where the row tiles alone do not fill the card: about four workgroups for each CU.
+  const int64_t group = q_heads / kv_heads;
+  // Rows of a sequence, on average.
+  const int64_t rows = ragged ? q_tokens * group / (batch > 0 ? batch : 1) : group;
+  p.query_tiles = rows <= 64 ? 1 : 0;
+  p.tile_rows = p.query_tiles > 0 ? kRows * p.query_tiles : kWaves * kRows;
+  p.row_tiles = ragged ? q_tokens * group / p.tile_rows + batch + 2
+                       : batch * ((group + p.tile_rows - 1) / p.tile_rows);
+  // Splits of the keys, so that there are about eight workgroups for each CU: sequences differ in length, and
+  // many short workgroups even that out.
   const int64_t base = p.row_tiles * kv_heads;
-  int64_t want = (4 * (int64_t)cus + base - 1) / base;
-  const int64_t least = kWaves * kTile * 2;
+  const int64_t want = (kStepGroups * (int64_t)cus + base - 1) / base;
   int64_t chunk = (most + want - 1) / want;
-  chunk = (chunk + kTile - 1) / kTile * kTile;
+  chunk = (chunk + kWaves * kTile - 1) / (kWaves * kTile) * (kWaves * kTile);
+  const int64_t least = kWaves * kTile * 2;
   if (chunk < least) chunk = least;
   p.chunk = (int32_t)chunk;
   p.splits = (int32_t)((most + chunk - 1) / chunk);
@@ -531,10 +1000,13 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
 template <int D, int FMT, int DT>
 void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   const dim3 grid((uint32_t)(a.kv_heads * p.row_tiles * a.splits));
-  hipLaunchKernelGGL((mx_attention_kernel<D, FMT, DT>), grid, dim3(kWaves * 64), 0, st, a);
+  if (p.query_tiles == 1)
+    hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 1>), grid, dim3(kWaves * 64), 0, st, a);
+  else
+    hipLaunchKernelGGL((mx_attention_kernel<D, FMT, DT>), grid, dim3(kWaves * 64), 0, st, a);
   if (a.splits > 1)
-    hipLaunchKernelGGL((mx_attention_join_kernel<DT>), dim3((uint32_t)a.q_tokens * (uint32_t)a.q_heads),
-                       dim3(256), 0, st, a, D);
+    hipLaunchKernelGGL((mx_attention_join_kernel<D, DT>), dim3((uint32_t)a.q_tokens * (uint32_t)a.q_heads),
+                       dim3(256), 0, st, a);
 }
 
 template <int FMT, int DT>
@@ -669,6 +1141,7 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   while (((int64_t)1 << a.page_shift) < page_size) ++a.page_shift;
   a.causal = causal != 0 ? 1 : 0;
   a.row_tiles = (int32_t)p.row_tiles;
+  a.tile_rows = p.tile_rows;
   a.chunk = p.chunk;
   a.splits = p.splits;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634074);
