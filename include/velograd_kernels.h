@@ -372,7 +372,8 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
  */
 VELOGRAD_API size_t velograd_mx_cache_attention_workspace_bytes(
     int64_t q_tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-    int64_t table_width, int64_t page_size, int32_t ragged, int32_t device);
+    int64_t table_width, int64_t page_size, int32_t ragged, int32_t dtype, int32_t mx_format,
+    int32_t device);
 
 /* Text of the calling thread's last error ("" if none).  No counterpart in the reference. */
 VELOGRAD_API const char* velograd_kernels_last_error(void);

@@ -79,22 +79,28 @@ def attention(q, parts, table, lengths, starts, page, fmt, scale, causal, out_ep
         pages = np.where(there, pages, 0)
         k = values(kc[pages, :, t % page], ks[pages, :, :, t % page], fmt)
         v = values(vc[pages, :, t % page], vs[pages, :, :, t % page], fmt)
-        for i in range(first, last):
-            limit = held - (last - first) + (i - first) + 1 if causal else held
-            seen = np.nonzero(there & (t < limit))[0]
-            if not len(seen):
-                continue
-            for h in range(heads):
-                kk, vv = k[seen, h // group], v[seen, h // group]
-                s = kk @ q[i, h] * scale
-                m = s.max()
-                p = np.exp(s - m)
-                total = p.sum()
-                out[i, h] = p @ vv / total
-                lse[i, h] = m + math.log(total)
-                weight = p @ np.abs(vv) / total
-                size = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
-                score = (dim + 12) * u * size
-                off[i, h] = out_eps * np.abs(out[i, h]) + weight * (p_eps + 2 * score + 4 * u + (len(seen) + 64) * u)
-                lse_off[i, h] = 2 * u * abs(lse[i, h]) + score + 4 * u + (len(seen) + 64) * u
+        if last == first or not held:
+            continue
+        limit = np.maximum(held - (last - first) + np.arange(last - first) + 1, 0) if causal else \
+            np.full(last - first, held)
+        hidden = ~there | (t >= limit[:, None])                       # [rows, keys]
+        seen = (~hidden).sum(-1)
+        rows = np.nonzero(seen)[0]
+        for h in range(heads):
+            kk, vv, qq = k[:, h // group], v[:, h // group], q[first:last, h][rows]
+            kk, vv = (np.where(there[:, None], x, 0.0) for x in (kk, vv))   # leftovers, NaN among them
+            s = np.where(hidden[rows], -np.inf, qq @ kk.T * scale)
+            m = s.max(-1, keepdims=True)
+            p = np.exp(s - m)
+            total = p.sum(-1, keepdims=True)
+            o = p @ vv / total
+            at = first + rows
+            out[at, h] = o
+            lse[at, h] = (m + np.log(total))[:, 0]
+            weight = p @ np.abs(vv) / total
+            size = np.where(hidden[rows], 0.0, np.abs(qq) @ np.abs(kk).T).max(-1) * abs(scale)
+            score = ((dim + 12) * u * size)[:, None]
+            sums = (seen[rows][:, None] + 64) * u
+            off[at, h] = out_eps * np.abs(o) + weight * (p_eps + 2 * score + 4 * u + sums)
+            lse_off[at, h] = (2 * u * np.abs(m + np.log(total)) + score + 4 * u + sums)[:, 0]
     return out, lse, off, lse_off

@@ -212,6 +212,8 @@ def test_no_tokens_is_a_no_op(lib):
 
 def test_workspace_of_bad_arguments_is_zero(lib):
     f = lib.velograd_mx_cache_attention_workspace_bytes
-    assert f(4, 4, 3, 2, 64, 2, 16, 0, 0) == 0
-    assert f(4, 4, 4, 2, 65, 2, 16, 0, 0) == 0
-    assert f(4, 5, 4, 2, 64, 2, 16, 0, 0) == 0
+    assert f(4, 4, 3, 2, 64, 2, 16, 0, 2, 1, 0) == 0
+    assert f(4, 4, 4, 2, 65, 2, 16, 0, 2, 1, 0) == 0
+    assert f(4, 5, 4, 2, 64, 2, 16, 0, 2, 1, 0) == 0
+    assert f(4, 4, 4, 2, 64, 2, 16, 0, 9, 1, 0) == 0
+    assert f(4, 4, 4, 2, 64, 2, 16, 0, 2, 9, 0) == 0

@@ -170,7 +170,7 @@ SIGNATURES = {
         _c_size,
         [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64,  # q_tokens, sequences, q_heads, kv_heads, head_dim
          _c_i64, _c_i64,                    # table_width, page_size
-         _c_i32, _c_i32],                   # ragged, device
+         _c_i32, _c_i32, _c_i32, _c_i32],   # ragged, dtype, mx_format, device
     ),
     "velograd_kernels_last_error": (ctypes.c_char_p, []),
     "velograd_kernels_version": (ctypes.c_char_p, []),

@@ -15,13 +15,12 @@
 // sums and outputs are held in fp32.
 //
 // The products are laid out so that nothing crosses lanes.  A lane is (n = lane % 16, g = lane / 16).
-//   S^T = K Q^T: A = K, row n of 16-token tile u holds token 8 (n / 4) + n % 4 + 4 u of the 32; the
-//     contraction's order is free, so lane g takes dims g D/4 .. (g + 1) D/4 - 1: whole MX blocks, one
-//     contiguous load.  B = Q^T, column n = query row.  The result's lane holds query row n and tokens
-//     8 g + (0..3) of tile 0 and 8 g + (4..7) of tile 1:
-//   O^T = V^T P^T: which is B's layout, P^T: column n, tokens 8 g .. 8 g + 7.  A = V^T: tile j's row n is
-//     dim n D/16 + j, so a lane decodes D/16 consecutive dims of 8 consecutive tokens, and pairs tokens
-//     by one byte permutation for each two elements.
+//   S^T = K Q^T: A = K, row n of half u of a 32-key tile is key 16 u + n; the contraction's order is free, so
+//     lane g takes chunks of 16 bytes g, g + 4, ..: each within an MX block, and four lanes' load contiguous.
+//     B = Q^T, column n = query row.  The result's lane holds query row n and keys 16 u + 4 g + (0..3):
+//   O^T = V^T P^T: which is B's layout, P^T: column n, with the contraction's 8 positions of lane g those
+//     keys.  A = V^T: fragment j's row n is dim n D/16 + j, so a lane decodes D/16 consecutive dims of its 8
+//     keys, and pairs keys by one byte permutation for each two elements.
 //   A query row's maximum, sum and rescaling are its lane's own (the four g's share the maximum).
 #include "mx_device.h"
 
@@ -32,10 +31,24 @@ using namespace vg;
 constexpr int kTile = 32;   // keys of one step
 constexpr int kWaves = 4;   // waves of a workgroup
 constexpr int kRows = 16;   // query rows of a wave
-#ifndef VG_STEP_GROUPS
-#define VG_STEP_GROUPS 8
+#ifndef VG_CHUNK_OCC
+#define VG_CHUNK_OCC 1
 #endif
-constexpr int kStepGroups = VG_STEP_GROUPS;
+#ifndef VG_CHUNK_NQ
+#define VG_CHUNK_NQ 4
+#endif
+// Query tiles of a wave at most, so that its rows and their sums fit the registers.
+constexpr int most_tiles(int dim, int dtype) {
+  const int tiles = dtype == VELOGRAD_DTYPE_BF16 ? VG_CHUNK_NQ : dtype == VELOGRAD_DTYPE_F16 ? 4 : 2;
+  return dim == 256 ? (dtype == VELOGRAD_DTYPE_BF16 ? 2 : 1) : dim == 128 && dtype == VELOGRAD_DTYPE_F16 ? 2 : tiles;
+}
+// Parts of a probability in chunks: the products count there, and one part of 8 bits (off by at most 2^-8 of
+// each probability, which average out over the keys) is as exact as the bf16 output.
+constexpr int chunk_parts(int dtype) {
+  return dtype == VELOGRAD_DTYPE_BF16 ? 1 : dtype == VELOGRAD_DTYPE_F16 ? 2 : 3;
+}
+
+constexpr int kLeastSteps = 4;  // of a wave's share
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -48,16 +61,18 @@ struct AttnArgs {
   const int32_t* starts;   // NULL: one new token for each sequence
   void* out;
   float* lse;              // may be NULL
-  float* part_o;           // [q_tokens * q_heads, splits, dim] when splits > 1
-  float* part_ml;          // [q_tokens * q_heads, splits, 2]
+  float* part_o;           // [workers, 2, tile_rows, dim]: unfinished sums
+  float* part_ml;          // [workers, 2, tile_rows, 2]: their maximum and sum
+  int32_t* joins;          // [q_tokens * q_heads, 2]: where a row's sums begin, and how many there are
   int64_t q_t, q_h;        // strides of q in elements
   int64_t table_stride;
   int32_t q_tokens, batch, q_heads, kv_heads, group;
   int32_t width;           // pages of a row of the table
   int32_t pages, page_shift;
   int32_t causal;
-  int32_t row_tiles, tile_rows;
-  int32_t chunk, splits;   // keys of a split (a multiple of kTile), splits of the longest sequence
+  int32_t workers;         // waves of the step kernel
+  int32_t least_steps;     // its smallest share
+  int32_t step_rows;       // sequences of more rows are the chunk kernel's
   float scale_log2;        // scale * log2(e)
 };
 
@@ -77,19 +92,6 @@ __device__ inline int32_t row_bound(const AttnArgs& a, int32_t i) {
   return x < 0 ? 0 : (x > a.q_tokens ? a.q_tokens : x);
 }
 
-// The last i of 0 .. batch + 1 with floor(bounds(i) * scale / tile) + (count ? i : 0) <= at, 64 bounds a
-// step.
-__device__ inline int32_t find_bound(const AttnArgs& a, int32_t scale, int32_t tile, bool count, int32_t at) {
-  const int32_t lane = threadIdx.x & 63;
-  int32_t n = 0;
-  for (int32_t i0 = 0; i0 < a.batch + 2; i0 += 64) {
-    const int32_t i = i0 + lane;
-    const bool below = i < a.batch + 2 && row_bound(a, i) * scale / tile + (count ? i : 0) <= at;
-    n += __popcll(__ballot(below));
-  }
-  return n - 1;
-}
-
 __device__ inline int32_t held_tokens(const AttnArgs& a, int32_t seq) {
   if (seq < 0 || seq >= a.batch) return 0;
   const int64_t most = (int64_t)a.width << a.page_shift;
@@ -97,21 +99,22 @@ __device__ inline int32_t held_tokens(const AttnArgs& a, int32_t seq) {
   return (int32_t)(x < 0 ? 0 : (x > most ? most : x));
 }
 
-__device__ inline RowTile find_tile(const AttnArgs& a, int32_t tile, int32_t tile_rows) {
+// Sequence i of a call as the kernels count them: with q_starts, i = 0 and i = batch + 1 are the rows before
+// the first sequence and behind the last.
+__device__ inline int32_t sequences(const AttnArgs& a) { return a.starts == nullptr ? a.batch : a.batch + 2; }
+
+__device__ inline RowTile sequence_rows(const AttnArgs& a, int32_t i) {
   RowTile r;
   if (a.starts == nullptr) {
-    const int32_t per = (a.group + tile_rows - 1) / tile_rows;
-    r.seq = tile / per;
-    r.row0 = (tile - r.seq * per) * tile_rows;
-    r.tok0 = r.seq;
+    r.seq = r.tok0 = i;
     r.fresh = 1;
   } else {
-    const int32_t i = find_bound(a, a.group, tile_rows, true, tile);
+    r.seq = i - 1 < a.batch ? i - 1 : -1;
     r.tok0 = row_bound(a, i);
     r.fresh = row_bound(a, i + 1) - r.tok0;
-    r.row0 = (tile - (r.tok0 * a.group / tile_rows + i)) * tile_rows;
-    r.seq = i - 1 < a.batch ? i - 1 : -1;
+    if (r.fresh < 0) r.fresh = 0;  // starts that fall: no rows
   }
+  r.row0 = 0;
   r.rows = r.fresh * a.group;
   r.length = held_tokens(a, r.seq);
   return r;
@@ -122,11 +125,6 @@ __device__ inline int32_t row_limit(const AttnArgs& a, const RowTile& r, int32_t
   int32_t x = a.causal ? r.length - r.fresh + i + 1 : r.length;
   if (x > r.length) x = r.length;
   return x < 0 ? 0 : x;
-}
-
-// Splits that a tile whose rows see up to `limit` keys has.
-__device__ inline int32_t splits_of(const AttnArgs& a, int32_t limit) {
-  return limit <= a.chunk ? 1 : (limit + a.chunk - 1) / a.chunk;
 }
 
 // Elements 2 SEL and 2 SEL + 1 of a word of codes, times 2^(scale's exponent), as a bf16 pair.
@@ -209,10 +207,12 @@ struct Shape {
   static constexpr int kSteps = D / 32;                              // products of S^T
   static constexpr int kOut = D / 16;                                // 16-dim tiles of O^T
   static constexpr int kRowBytes = FMT == VELOGRAD_MX_E2M1 ? D / 2 : D;
-  static constexpr int kKBytes = kRowBytes / 4;                      // a lane's bytes of a key
+  static constexpr int kKBytes = kRowBytes / 4;                      // a lane's bytes of a key,
+  static constexpr int kChunkBytes = kKBytes < 16 ? kKBytes : 16;    // in chunks, 4 lanes' side by side
+  static constexpr int kChunks = kKBytes / kChunkBytes;
+  static constexpr int kChunkElems = FMT == VELOGRAD_MX_E2M1 ? 2 * kChunkBytes : kChunkBytes;  // 16 or 32
   static constexpr int kVBytes = kRowBytes / 16;                     // a lane's bytes of a value
   static constexpr int kPerWord = FMT == VELOGRAD_MX_E2M1 ? 4 : 2;   // pairs in a word of codes
-  static constexpr int kKScales = D / 4 >= 32 ? D / 128 : 1;         // blocks of a lane's part of a key
   static constexpr int kQParts = DT == VELOGRAD_DTYPE_BF16 ? 1 : DT == VELOGRAD_DTYPE_F16 ? 2 : 3;
   static constexpr int kPParts = DT == VELOGRAD_DTYPE_F32 ? 3 : 2;
 };
@@ -237,327 +237,70 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-template <int D, int FMT, int DT>
-__global__ __launch_bounds__(kWaves * 64) void mx_attention_kernel(const AttnArgs a) {
-  using S = Shape<D, FMT, DT>;
-  constexpr int kWordsK = S::kKBytes / 4;
-  constexpr int kWordsV = S::kVBytes < 4 ? 1 : S::kVBytes / 4;
-  // Heads fastest, then row tiles, then splits.
-  const uint32_t tile_split = blockIdx.x / (uint32_t)a.kv_heads;
-  const int32_t h = (int32_t)(blockIdx.x - tile_split * (uint32_t)a.kv_heads);
-  const int32_t split = (int32_t)(tile_split / (uint32_t)a.row_tiles);
-  const RowTile r = find_tile(a, (int32_t)(tile_split - (uint32_t)split * (uint32_t)a.row_tiles), kWaves * kRows);
-  if (r.row0 < 0 || r.row0 >= r.rows) return;
-  const int32_t here = r.rows - r.row0 < kWaves * kRows ? r.rows - r.row0 : kWaves * kRows;
-  // Few rows: all waves take the same ones and share the keys out; else every wave takes its own.
-  const bool share = here <= kRows;
-  const int32_t wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const int32_t wrow = share ? r.row0 : r.row0 + wave * kRows;
-  const int32_t tile_limit = row_limit(a, r, (r.row0 + here - 1) / a.group);
-  const int32_t active = splits_of(a, tile_limit);
-  if (split >= active) return;
-
-  const int32_t row = wrow + n;
-  const bool row_ok = row < r.rows;
-  const int32_t fresh = row_ok ? row / a.group : 0;
-  const int32_t head = h * a.group + (row_ok ? row - fresh * a.group : 0);
-  const int32_t limit = row_ok ? row_limit(a, r, fresh) : 0;
-  const int64_t tok = r.tok0 + fresh;
-
-  // The query row's fragments: dims g D/4 + 8 s .. + 7 for product s.
-  u32x4 qf[S::kSteps][S::kQParts];
-#pragma unroll
-  for (int s = 0; s < S::kSteps; ++s) {
-    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (row_ok) {
-      const int64_t e = tok * a.q_t + head * a.q_h + g * (D / 4) + 8 * s;
-      Codec<DT>::unpack(load16_any<DT>(a.q, e), f);
-      if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, e + 4), f + 4);
-    }
-    split_parts<S::kQParts>(f, qf[s]);
-  }
-
-  f32x4 acc[S::kOut];
-#pragma unroll
-  for (int j = 0; j < S::kOut; ++j) acc[j] = f32x4{0, 0, 0, 0};
-  float m = -3.0e38f, l = 0.0f;
-
-  // The wave's keys: [begin, end) in steps; all its rows see every key below `clear`.
-  int32_t end = (split + 1) * a.chunk;
-  const int32_t last_row = (wrow + kRows < r.rows ? wrow + kRows : r.rows) - 1;
-  const int32_t wave_limit = wrow < r.rows ? row_limit(a, r, last_row / a.group) : 0;
-  if (end > wave_limit) end = wave_limit;
-  const int32_t clear = wrow < r.rows ? row_limit(a, r, wrow / a.group) : 0;
-  const int32_t begin = split * a.chunk + (share ? wave * kTile : 0);
-  const int32_t stride = share ? kWaves * kTile : kTile;
-  const int32_t* table = a.table + (int64_t)(r.seq < 0 ? 0 : r.seq) * a.table_stride;
-  const int32_t page_mask = (1 << a.page_shift) - 1;
-
-  for (int32_t t0 = begin; t0 < end; t0 += stride) {
-    const int32_t tk = t0 + 8 * (n >> 2) + (n & 3), tv = t0 + 8 * g;
-    int32_t ik = tk >> a.page_shift, iv = tv >> a.page_shift;
-    if (ik >= a.width) ik = a.width - 1;
-    if (iv >= a.width) iv = a.width - 1;
-    int32_t pk = table[ik], pv = table[iv];
-    const bool bad = (uint32_t)pv >= (uint32_t)a.pages;
-    if ((uint32_t)pk >= (uint32_t)a.pages) pk = 0;
-    if (bad) pv = 0;
-    const int64_t hk = (int64_t)pk * a.kv_heads + h, hv = (int64_t)pv * a.kv_heads + h;
-    const int32_t ok = tk & page_mask, ov = tv & page_mask;
-
-    const uint8_t* kp = a.kc + ((hk << a.page_shift) + ok) * S::kRowBytes + g * S::kKBytes;
-    const uint8_t* vp = a.vc + ((hv << a.page_shift) + ov) * S::kRowBytes + n * S::kVBytes;
-    uint32_t kw[2][kWordsK], vw[8][kWordsV], kscale[2][S::kKScales];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      load_words<S::kKBytes>(kp + 4 * u * S::kRowBytes, kw[u]);
-#pragma unroll
-      for (int b = 0; b < S::kKScales; ++b)
-        kscale[u][b] = a.ks[((hk * (D / 32) + (g * (D / 4)) / 32 + b) << a.page_shift) + ok + 4 * u];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) load_words<S::kVBytes>(vp + i * S::kRowBytes, vw[i]);
-    u32x2 vscale = *reinterpret_cast<const u32x2*>(
-        a.vs + ((hv * (D / 32) + (n * (D / 16)) / 32) << a.page_shift) + ov);
-
-    // Scores.
-    f32x4 sc[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc[u] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int s = 0; s < S::kSteps; ++s) {
-        u32x4 kf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pair = 4 * s + i;  // of the lane's D/8 pairs
-          kf[i] = decode_pair<FMT>(kw[u][pair / S::kPerWord], scale_arg(kscale[u][pair / 16 % S::kKScales]),
-                                   pair % S::kPerWord);
-        }
-#pragma unroll
-        for (int p = S::kQParts - 1; p >= 0; --p) sc[u] = mfma(kf, qf[s][p], sc[u]);
-      }
-    }
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = sc[i >> 2][i & 3] * a.scale_log2;
-
-    const bool masked = t0 + kTile > clear || __ballot(bad) != 0;
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (bad || tv + i >= limit) x[i] = -__builtin_inff();
-        // Nothing is read of what lies behind the sequence's end: its codes may be anything.
-        if (bad || tv + i >= r.length) {
-#pragma unroll
-          for (int w = 0; w < kWordsV; ++w) vw[i][w] = 0;
-          vscale[i >> 2] = (vscale[i >> 2] & ~(0xffu << (8 * (i & 3)))) | (127u << (8 * (i & 3)));
-        }
-      }
-    }
-
-    // The running maximum moves only when a row's new maximum passes it by 8 (p stays below 2^8, which
-    // costs fp32 nothing): most steps rescale nothing.
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
-    if (__ballot(top > m + 8.0f) != 0) {
-      top = across_g(top, false);
-      const float next = top > m + 8.0f ? top : m;  // for each row by itself
-      const float f = __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      l *= f;
-#pragma unroll
-      for (int j = 0; j < S::kOut; ++j) acc[j] *= f;
-    }
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(x[i] - m);
-      l += p[i];
-    }
-    u32x4 pf[S::kPParts];
-    split_parts<S::kPParts>(p, pf);
-
-    // Values: dims n D/16 + j of tokens 8 g .. 8 g + 7.
-    u32x4 vf[S::kOut];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float s0 = scale_arg(vscale[i >> 1] >> (16 * (i & 1)));
-      const float s1 = scale_arg(vscale[i >> 1] >> (16 * (i & 1) + 8));
-#pragma unroll
-      for (int d = 0; d < S::kOut / 2; ++d) {
-        const uint32_t u0 = decode_pair<FMT>(vw[2 * i][d / S::kPerWord], s0, d % S::kPerWord);
-        const uint32_t u1 = decode_pair<FMT>(vw[2 * i + 1][d / S::kPerWord], s1, d % S::kPerWord);
-        vf[2 * d][i] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
-        vf[2 * d + 1][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-      }
-    }
-    if (masked && a.causal) {
-      // A NaN among the values of a key that only some of the rows see would reach the others as 0 * NaN:
-      // it is taken out of the product, and the rows that do see it get NaN by a product of flags.
-      bool any = false;
-#pragma unroll
-      for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          any |= (vf[j][i] & 0x7fffu) > 0x7f80u || (vf[j][i] & 0x7fff0000u) > 0x7f800000u;
-      if (__ballot(any) != 0) {
-        u32x4 seen;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          seen[i] = (x[2 * i] != -__builtin_inff() ? 0x3f80u : 0u) |
-                    (x[2 * i + 1] != -__builtin_inff() ? 0x3f800000u : 0u);
-#pragma unroll
-        for (int j = 0; j < S::kOut; ++j) {
-          u32x4 flag;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool lo = (vf[j][i] & 0x7fffu) > 0x7f80u, hi = (vf[j][i] & 0x7fff0000u) > 0x7f800000u;
-            flag[i] = (lo ? 0x3f80u : 0u) | (hi ? 0x3f800000u : 0u);
-            vf[j][i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-          }
-          const f32x4 hit = mfma(flag, seen, f32x4{0, 0, 0, 0});
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hit[i] > 0.0f) acc[j][i] = __builtin_nanf("");
-        }
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-      for (int q = S::kPParts - 1; q >= 0; --q) acc[j] = mfma(vf[j], pf[q], acc[j]);
-  }
-
-  if (share) {
-    // Waves 2, 3 hand their sums to 0, 1, then 1 to 0, in the accumulators' own layout.
-    __shared__ float buf[kWaves / 2][D / 4 + 2][64];
-#pragma unroll
-    for (int w = kWaves / 2; w >= 1; w >>= 1) {
-      if (wave >= w && wave < 2 * w) {
-#pragma unroll
-        for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) buf[wave - w][4 * j + i][lane] = acc[j][i];
-        buf[wave - w][D / 4][lane] = m;
-        buf[wave - w][D / 4 + 1][lane] = l;
-      }
-      __syncthreads();
-      if (wave < w) {
-        const float mo = buf[wave][D / 4][lane];
-        const float next = __builtin_fmaxf(m, mo);
-        const float f = __builtin_amdgcn_exp2f(m - next), fo = __builtin_amdgcn_exp2f(mo - next);
-        m = next;
-        l = l * f + buf[wave][D / 4 + 1][lane] * fo;
-#pragma unroll
-        for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][i] = acc[j][i] * f + buf[wave][4 * j + i][lane] * fo;
-      }
-      __syncthreads();
-    }
-    if (wave != 0) return;
-  }
-  l = across_g(l, true);
-  if (!row_ok) return;
-  const int64_t orow = tok * a.q_heads + head;
-  if (active > 1) {
-    float* po = a.part_o + (orow * a.splits + split) * D;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < S::kOut; ++j) po[(4 * g + i) * S::kOut + j] = acc[j][i];
-    if (g == 0) {
-      a.part_ml[(orow * a.splits + split) * 2] = m;
-      a.part_ml[(orow * a.splits + split) * 2 + 1] = l;
-    }
-    return;
-  }
-  const bool empty = l == 0.0f;
-  const float inv = empty ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < S::kOut; ++j)
-      Codec<DT>::store1(a.out, orow * D + (4 * g + i) * S::kOut + j, empty ? 0.0f : acc[j][i] * inv);
-  if (a.lse != nullptr && g == 0)
-    a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(l)) * 0.693147180559945309f;
-}
-
 // ------------------------------------------------------------------------------------------
 // Few rows a sequence: single and drafted tokens.
 // ------------------------------------------------------------------------------------------
-// A workgroup's four waves take the same 16 NQ query rows, each a quarter of the split's keys in one run,
-// and add up at the end through LDS.  A wave reads its keys' codes straight into registers, one step of 32
-// ahead of the products.  Page numbers come from one load of a lane each for 64 groups of 8 keys (512
-// keys), and reach the addresses as scalars: a step's two halves of 16 keys lie on one page each.
-constexpr int kRunGroups = 64;
-constexpr int kRunKeys = 8 * kRunGroups;
+// Every wave works by itself, on 16 NQ query rows of one kv head and a run of keys at a time, and reads the
+// keys' codes straight into registers, one step of 32 ahead of the products.  Pages are looked up once for
+// 1024 keys, by each lane for the 16 keys of a half step, which one page holds; a step takes its two halves'
+// offsets from those lanes as scalars.
+constexpr int kHalf = kTile / 2;
+constexpr int kRunKeys = 64 * kHalf;
 
 template <int D, int FMT>
 struct KeyTile {
   using S = Shape<D, FMT, VELOGRAD_DTYPE_BF16>;
   static constexpr int kWordsK = S::kKBytes / 4;
   static constexpr int kWordsV = S::kVBytes < 4 ? 1 : S::kVBytes / 4;
-  uint32_t kw[2][kWordsK];
-  uint32_t ks[2][S::kKScales];
-  uint32_t vw[8][kWordsV];
+  uint32_t kw[2][kWordsK];       // key n of each half: a lane's parts
+  uint32_t ks[2][S::kChunks];    // and their scales
+  uint32_t vw[8][kWordsV];       // values 4 g + (0..3) of each half
   u32x2 vs;
 };
 
-struct CacheView {
-  const uint8_t *kc, *ks, *vc, *vs;  // of the head
-  int64_t code_page, scale_page;     // bytes of a page, all heads
-  int32_t page_shift;
+// Byte offsets of a lane's parts from the first key of a half tile.
+struct LaneView {
+  uint32_t k, ks, v, vs;
 };
 
-// Keys t .. t + 31, whose halves lie on pages p0 and p1 (places a0 and a1 of them).
+// A half's codes and scales; the addresses are the half's, the same for the wave, and the lane's own 32 bits.
 template <int D, int FMT>
-__device__ __forceinline__ void load_tile(const CacheView& c, int32_t p0, int32_t a0, int32_t p1, int32_t a1,
-                                          int32_t n, int32_t g, KeyTile<D, FMT>& t) {
+__device__ __forceinline__ void load_half(const AttnArgs& a, const LaneView& c, int64_t code, int64_t scale, int u,
+                                          KeyTile<D, FMT>& t) {
   using S = typename KeyTile<D, FMT>::S;
-  const int64_t c0 = p0 * c.code_page + (int64_t)a0 * S::kRowBytes, c1 = p1 * c.code_page + (int64_t)a1 * S::kRowBytes;
-  const int64_t s0 = p0 * c.scale_page + a0, s1 = p1 * c.scale_page + a1;
-  const int32_t gk = n >> 2;  // the lane's group of 8 keys, as a row of K
-  const uint8_t* kp = c.kc + (gk & 2 ? c1 : c0) + (8 * (gk & 1) + (n & 3)) * S::kRowBytes + g * S::kKBytes;
-  const uint8_t* kq = c.ks + (gk & 2 ? s1 : s0) + (((g * (D / 4)) / 32) << c.page_shift) + 8 * (gk & 1) + (n & 3);
-  const uint8_t* vp = c.vc + (g & 2 ? c1 : c0) + 8 * (g & 1) * S::kRowBytes + n * S::kVBytes;
-  const uint8_t* vq = c.vs + (g & 2 ? s1 : s0) + (((n * (D / 16)) / 32) << c.page_shift) + 8 * (g & 1);
+  const uint8_t *kp = a.kc + code, *vp = a.vc + code, *kq = a.ks + scale, *vq = a.vs + scale;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    load_words<S::kKBytes>(kp + 4 * u * S::kRowBytes, t.kw[u]);
-#pragma unroll
-    for (int b = 0; b < S::kKScales; ++b) t.ks[u][b] = kq[((int64_t)b << c.page_shift) + 4 * u];
+  for (int i = 0; i < S::kChunks; ++i) {
+    load_words<S::kChunkBytes>(kp + (c.k + 4 * i * S::kChunkBytes), t.kw[u] + i * (S::kChunkBytes / 4));
+    t.ks[u][i] = kq[c.ks + (uint32_t)((i * (S::kChunkElems / 8)) << a.page_shift)];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load_words<S::kVBytes>(vp + i * S::kRowBytes, t.vw[i]);
-  t.vs = *reinterpret_cast<const u32x2*>(vq);
+  for (int i = 0; i < 4; ++i) load_words<S::kVBytes>(vp + (c.v + i * S::kRowBytes), t.vw[4 * u + i]);
+  t.vs[u] = *reinterpret_cast<const uint32_t*>(vq + c.vs);
 }
 
-// S^T of the tile for one query tile: x[i] is the score of key 8 g + i, unscaled.
-template <int D, int FMT, int PARTS>
+// K of the tile: fragment s of half u holds elements 8 s .. 8 s + 7 of the lane's part of key n.
+template <int D, int FMT>
 __device__ __forceinline__ void decode_keys(const KeyTile<D, FMT>& t, u32x4 (*kf)[D / 32]) {
   using S = typename KeyTile<D, FMT>::S;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    float scale[S::kKScales];
+    float scale[S::kChunks];
 #pragma unroll
-    for (int b = 0; b < S::kKScales; ++b) scale[b] = scale_arg(t.ks[u][b]);
+    for (int b = 0; b < S::kChunks; ++b) scale[b] = scale_arg(t.ks[u][b]);
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int pair = 4 * s + i;  // of the lane's D/8 pairs
-        kf[u][s][i] = decode_pair<FMT>(t.kw[u][pair / S::kPerWord], scale[pair / 16 % S::kKScales], pair % S::kPerWord);
+        kf[u][s][i] = decode_pair<FMT>(t.kw[u][pair / S::kPerWord], scale[8 * s / S::kChunkElems], pair % S::kPerWord);
       }
   }
 }
 
-// V^T of the tile: fragment j is dim n D/16 + j of keys 8 g .. 8 g + 7.
+// Fragments 2 d and 2 d + 1 of V^T of the tile: dims n D/16 + 2 d, + 1 of the lane's 8 keys.
 template <int D, int FMT>
-__device__ __forceinline__ void decode_values(const KeyTile<D, FMT>& t, u32x4* vf) {
+__device__ __forceinline__ void decode_values(const KeyTile<D, FMT>& t, int d, u32x4* vf) {
   using S = typename KeyTile<D, FMT>::S;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -565,13 +308,10 @@ __device__ __forceinline__ void decode_values(const KeyTile<D, FMT>& t, u32x4* v
     const uint32_t w = t.vs[i >> 1];
     const float s0 = __builtin_bit_cast(float, i & 1 ? w << 7 : w << 23);
     const float s1 = __builtin_bit_cast(float, i & 1 ? w >> 1 : w << 15);
-#pragma unroll
-    for (int d = 0; d < S::kOut / 2; ++d) {
-      const uint32_t u0 = decode_pair<FMT>(t.vw[2 * i][d / S::kPerWord], s0, d % S::kPerWord);
-      const uint32_t u1 = decode_pair<FMT>(t.vw[2 * i + 1][d / S::kPerWord], s1, d % S::kPerWord);
-      vf[2 * d][i] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
-      vf[2 * d + 1][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-    }
+    const uint32_t u0 = decode_pair<FMT>(t.vw[2 * i][d / S::kPerWord], s0, d % S::kPerWord);
+    const uint32_t u1 = decode_pair<FMT>(t.vw[2 * i + 1][d / S::kPerWord], s1, d % S::kPerWord);
+    vf[0][i] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
+    vf[1][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
   }
 }
 
@@ -668,25 +408,27 @@ __device__ __forceinline__ void keep_nan_apart(KeyTile<D, FMT>& t, const float (
   for (int i = 0; i < 2; ++i) t.vs[i] &= ~(nan_scales(t.vs[i]));  // 0xFF -> 0x7F
 }
 
-// A row's result, unnormalised sums to the workspace where the keys are split, else out and lse.
-template <int D, int DT>
-__device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& r, int64_t orow, int32_t split,
-                                          bool partial, int32_t g) {
+// A row's unfinished sums, into row `at` of the workspace's [.., tile_rows, D].
+template <int D>
+__device__ __forceinline__ void store_part(const AttnArgs& a, const RowState<D>& r, int64_t at, int32_t g) {
   constexpr int kOut = D / 16;
-  if (partial) {
-    float* po = a.part_o + (orow * a.splits + split) * D;
+  float* po = a.part_o + at * D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < kOut; j += 4)
-        *reinterpret_cast<f32x4*>(po + (4 * g + i) * kOut + j) =
-            f32x4{r.acc[j][i], r.acc[j + 1][i], r.acc[j + 2][i], r.acc[j + 3][i]};
-    if (g == 0) {
-      a.part_ml[(orow * a.splits + split) * 2] = r.m;
-      a.part_ml[(orow * a.splits + split) * 2 + 1] = r.l;
-    }
-    return;
+    for (int j = 0; j < kOut; j += 4)
+      *reinterpret_cast<f32x4*>(po + (4 * g + i) * kOut + j) =
+          f32x4{r.acc[j][i], r.acc[j + 1][i], r.acc[j + 2][i], r.acc[j + 3][i]};
+  if (g == 0) {
+    a.part_ml[at * 2] = r.m;
+    a.part_ml[at * 2 + 1] = r.l;
   }
+}
+
+// A row's out and lse.
+template <int D, int DT>
+__device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& r, int64_t orow, int32_t g) {
+  constexpr int kOut = D / 16;
   const bool empty = r.l == 0.0f;
   const float inv = empty ? 0.0f : 1.0f / r.l;
 #pragma unroll
@@ -707,105 +449,179 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
     a.lse[orow] = empty ? -__builtin_inff() : (r.m + log2f(r.l)) * 0.693147180559945309f;
 }
 
-// A query row's fragments: dims g D/4 + 8 s .. + 7 for product s; zeros for a row that is none.
-template <int D, int DT>
-__device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, bool ok,
-                                           u32x4 (*qf)[Shape<D, VELOGRAD_MX_E2M1, DT>::kQParts]) {
-  using S = Shape<D, VELOGRAD_MX_E2M1, DT>;
+// A query row's fragments, in the order of decode_keys; zeros for a row that is none.
+template <int D, int FMT, int DT>
+__device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, int32_t g, bool ok,
+                                           u32x4 (*qf)[Shape<D, FMT, DT>::kQParts]) {
+  using S = Shape<D, FMT, DT>;
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (ok) {
-      Codec<DT>::unpack(load16_any<DT>(a.q, e + 8 * s), f);
-      if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, e + 8 * s + 4), f + 4);
+      const int64_t at = e + (4 * (8 * s / S::kChunkElems) + g) * S::kChunkElems + 8 * s % S::kChunkElems;
+      Codec<DT>::unpack(load16_any<DT>(a.q, at), f);
+      if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, at + 4), f + 4);
     }
     split_parts<S::kQParts>(f, qf[s]);
   }
 }
 
-// Waves of a SIMD that the registers are held to: as many as take no spills.
-constexpr int step_occupancy(int dim, int fmt, int dtype) {
-  const bool small = fmt == VELOGRAD_MX_E2M1, plain = dtype == VELOGRAD_DTYPE_BF16;
-  return dim == 64 ? (small || plain ? 4 : 3) : dim == 128 ? (small && plain ? 3 : 2) : 1;
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+__device__ __forceinline__ int64_t take_lane(int64_t v, int32_t lane) {
+  const u32x2 w = __builtin_bit_cast(u32x2, v);
+  const u32x2 r = {(uint32_t)__builtin_amdgcn_readlane((int)w[0], lane),
+                   (uint32_t)__builtin_amdgcn_readlane((int)w[1], lane)};
+  return __builtin_bit_cast(int64_t, r);
 }
 
+// Steps of an item: a tile of rows of one kv head over everything its sequence holds.
+__device__ inline int32_t tile_steps(int32_t length) { return length <= kTile ? 1 : (length + kTile - 1) / kTile; }
+
+// A wave's share of a head's steps, in the order sequence, row tile, step.
+struct Share {
+  int32_t sequence, tile, step;        // where it begins
+  int32_t steps;                       // how many it has
+};
+
+__device__ inline int64_t sequence_steps(const AttnArgs& a, int32_t i, int32_t tile_rows) {
+  if (i >= sequences(a)) return 0;
+  const RowTile r = sequence_rows(a, i);
+  if (r.rows > a.step_rows) return 0;
+  return (int64_t)((r.rows + tile_rows - 1) / tile_rows) * tile_steps(r.length);
+}
+
+// Sequences differ in length, so a head's steps are dealt out in equal shares of consecutive ones, each to one
+// wave, whatever items they belong to; wave w takes head w % kv_heads, so neighbouring waves read the same
+// pages.  Every workgroup adds up all sequences' steps, and finds the sequences that its waves' shares begin
+// in.  Returns the steps of every share but the last.
+__device__ inline int32_t find_shares(const AttnArgs& a, int32_t tile_rows, Share* found) {
+  __shared__ int64_t sums[2][kWaves];
+  const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = kWaves * 64;
+  const int32_t count = sequences(a);
+  if (tid < kWaves) found[tid].steps = 0;
+  const int64_t mine = sequence_steps(a, tid, tile_rows);
+  int64_t total = mine;
+  for (int32_t i = tid + threads; i < count; i += threads) total += sequence_steps(a, i, tile_rows);
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) total += __shfl_xor(total, w);
+  if (lane == 0) sums[0][wave] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) total += sums[0][w];
+  const int32_t each = a.workers / a.kv_heads;  // shares of a head
+  int64_t share = (total + each - 1) / each;
+  if (share < a.least_steps) share = a.least_steps;
+  const int32_t worker = (int32_t)blockIdx.x * kWaves;
+  const int64_t begin = share * (worker / a.kv_heads), ending = share * ((worker + kWaves - 1) / a.kv_heads);
+  int64_t before = 0;  // steps before the sequences at hand
+  for (int32_t i0 = 0; i0 < count; i0 += threads) {
+    const int64_t one = i0 == 0 ? mine : sequence_steps(a, i0 + tid, tile_rows);
+    int64_t upto = one;  // inclusive, within the wave
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int64_t x = __shfl_up(upto, w);
+      if (lane >= w) upto += x;
+    }
+    if (i0 > 0) __syncthreads();
+    if (lane == 63) sums[1][wave] = upto;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) upto += sums[1][w];
+      all += sums[1][w];
+    }
+    const int64_t lo = before + upto - one, hi = before + upto;
+    if (hi > begin && lo <= ending && one > 0) {
+      const int32_t steps = tile_steps(held_tokens(a, a.starts == nullptr ? i0 + tid : i0 + tid - 1));
+#pragma unroll 1
+      for (int w = 0; w < kWaves; ++w) {
+        const int64_t from = share * ((worker + w) / a.kv_heads);
+        if (from < lo || from >= hi) continue;
+        found[w].sequence = i0 + tid;
+        found[w].tile = (int32_t)((from - lo) / steps);
+        found[w].step = (int32_t)(from - lo - (int64_t)found[w].tile * steps);
+        found[w].steps = (int32_t)(total - from < share ? total - from : share);
+      }
+    }
+    before += all;
+    if (before > ending) break;
+  }
+  __syncthreads();
+  return uniform((int32_t)share);
+}
+
+// A wave's query rows: 16 NQ rows of a tile, each in a lane's column.
 template <int D, int FMT, int DT, int NQ>
-__global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT)) void mx_attention_step_kernel(const AttnArgs a) {
-  using S = Shape<D, FMT, DT>;
-  constexpr int kTileRows = kRows * NQ;
-  // Heads fastest, then row tiles, then splits.
-  const uint32_t tile_split = blockIdx.x / (uint32_t)a.kv_heads;
-  const int32_t h = (int32_t)(blockIdx.x - tile_split * (uint32_t)a.kv_heads);
-  const int32_t split = (int32_t)(tile_split / (uint32_t)a.row_tiles);
-  const RowTile r = find_tile(a, (int32_t)(tile_split - (uint32_t)split * (uint32_t)a.row_tiles), kTileRows);
-  if (r.row0 < 0 || r.row0 >= r.rows) return;
-  const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
-  const int32_t most = row_limit(a, r, last / a.group);      // keys that the tile's last row sees,
-  const int32_t clear = row_limit(a, r, r.row0 / a.group);   // and that all its rows see
-  const int32_t active = splits_of(a, most);
-  if (split >= active) return;
-  const int32_t wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+struct QueryRows {
+  bool ok[NQ];
+  int32_t limit[NQ];   // keys that the row sees
+  int64_t orow[NQ];    // its row of the output
+  u32x4 frag[NQ][D / 32][Shape<D, FMT, DT>::kQParts];
+  RowState<D> state[NQ];
+};
+
+template <int D, int FMT, int DT, int NQ>
+__device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, int32_t h,
+                                           QueryRows<D, FMT, DT, NQ>& w) {
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-
-  // The wave's keys: a quarter of the split's steps.
-  const int32_t from = split * a.chunk;
-  const int32_t till = from + a.chunk < most ? from + a.chunk : most;
-  const int32_t steps = (till - from + kTile - 1) / kTile;
-  const int32_t begin = from + (steps * wave / kWaves) * kTile;
-  int32_t end = from + (steps * (wave + 1) / kWaves) * kTile;
-  if (end > till) end = till;
-
-  bool row_ok[NQ];
-  int32_t limit[NQ];
-  int64_t orow[NQ];
-  u32x4 qf[NQ][S::kSteps][S::kQParts];
-  RowState<D> rows[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const int32_t row = r.row0 + kRows * q + n;
-    row_ok[q] = row < r.rows;
-    const int32_t fresh = row_ok[q] ? row / a.group : 0;
-    const int32_t head = h * a.group + (row_ok[q] ? row - fresh * a.group : 0);
-    limit[q] = row_ok[q] ? row_limit(a, r, fresh) : 0;
+    w.ok[q] = row < r.rows;
+    const int32_t fresh = w.ok[q] ? row / a.group : 0;
+    const int32_t head = h * a.group + (w.ok[q] ? row - fresh * a.group : 0);
+    w.limit[q] = w.ok[q] ? row_limit(a, r, fresh) : 0;
     const int64_t tok = r.tok0 + fresh;
-    orow[q] = tok * a.q_heads + head;
-    load_query<D, DT>(a, tok * a.q_t + head * a.q_h + g * (D / 4), row_ok[q], qf[q]);
+    w.orow[q] = tok * a.q_heads + head;
+    load_query<D, FMT, DT>(a, tok * a.q_t + head * a.q_h, g, w.ok[q], w.frag[q]);
 #pragma unroll
-    for (int j = 0; j < S::kOut; ++j) rows[q].acc[j] = f32x4{0, 0, 0, 0};
-    rows[q].m = -3.0e38f;
-    rows[q].l = 0.0f;
+    for (int j = 0; j < D / 16; ++j) w.state[q].acc[j] = f32x4{0, 0, 0, 0};
+    w.state[q].m = -3.0e38f;
+    w.state[q].l = 0.0f;
   }
+}
 
-  const int32_t* table = a.table + (int64_t)(r.seq < 0 ? 0 : r.seq) * a.table_stride;
+// Keys from .. end - 1 (from a multiple of 32) of the tile's sequence and kv head h.  All rows see the keys
+// below `clear`, the last of them those below `most`.  PARTS: of the probabilities.
+template <int D, int FMT, int DT, int NQ, int PARTS>
+__device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int32_t h, int32_t from, int32_t end,
+                                       int32_t clear, int32_t most, QueryRows<D, FMT, DT, NQ>& rows) {
+  using S = Shape<D, FMT, DT>;
+  const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int32_t page_mask = (1 << a.page_shift) - 1;
-  CacheView c;
-  c.page_shift = a.page_shift;
-  c.code_page = (int64_t)a.kv_heads * S::kRowBytes << a.page_shift;
-  c.scale_page = (int64_t)a.kv_heads * (D / 32) << a.page_shift;
-  c.kc = a.kc + ((int64_t)h * S::kRowBytes << a.page_shift);
-  c.vc = a.vc + ((int64_t)h * S::kRowBytes << a.page_shift);
-  c.ks = a.ks + ((int64_t)h * (D / 32) << a.page_shift);
-  c.vs = a.vs + ((int64_t)h * (D / 32) << a.page_shift);
+  const int32_t* table = a.table + (int64_t)(r.seq < 0 ? 0 : r.seq) * a.table_stride;
+  LaneView c;
+  c.k = n * S::kRowBytes + g * S::kChunkBytes;
+  c.v = 4 * g * S::kRowBytes + n * S::kVBytes;
+  c.ks = (((g * S::kChunkElems) / 32) << a.page_shift) + n;
+  c.vs = (((n * (D / 16)) / 32) << a.page_shift) + 4 * g;
 
-  for (int32_t run = begin; run < end; run += kRunKeys) {
+  for (int32_t run = from; run < end; run += kRunKeys) {
     const int32_t run_end = run + kRunKeys < end ? run + kRunKeys : end;
-    int32_t at = (run + 8 * lane) >> a.page_shift;
+    int32_t at = (run + kHalf * lane) >> a.page_shift;
     if (at >= a.width) at = a.width - 1;
     int32_t page = table[at];
     const bool none = (uint32_t)page >= (uint32_t)a.pages;
     if (none) page = 0;
     const uint64_t missing = __ballot(none);
+    const int64_t paged = (int64_t)page * a.kv_heads + h;
+    const int32_t place = (run + kHalf * lane) & page_mask;
+    const int64_t code = ((paged << a.page_shift) + place) * S::kRowBytes;
+    const int64_t scale = ((paged * (D / 32)) << a.page_shift) + place;
 
     auto fetch = [&](int32_t t0, KeyTile<D, FMT>& t) {
-      const int32_t i = (t0 - run) >> 3;
-      const int32_t p0 = __builtin_amdgcn_readlane(page, i), p1 = __builtin_amdgcn_readlane(page, i + 2);
-      load_tile<D, FMT>(c, p0, t0 & page_mask, p1, (t0 + 16) & page_mask, n, g, t);
+      const int32_t i = (t0 - run) / kHalf;
+      load_half<D, FMT>(a, c, take_lane(code, i), take_lane(scale, i), 0, t);
+      load_half<D, FMT>(a, c, take_lane(code, i + 1), take_lane(scale, i + 1), 1, t);
     };
     auto use = [&](int32_t t0, KeyTile<D, FMT>& t) {
       float x[NQ][8];
       {
         u32x4 kf[2][S::kSteps];
-        decode_keys<D, FMT, S::kQParts>(t, kf);
+        decode_keys<D, FMT>(t, kf);
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -814,44 +630,55 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT)) void mx_at
 #pragma unroll
             for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
-              for (int p = S::kQParts - 1; p >= 0; --p) sc = mfma(kf[u][s], qf[q][s][p], sc);
+              for (int p = S::kQParts - 1; p >= 0; --p) sc = mfma(kf[u][s], rows.frag[q][s][p], sc);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[q][4 * u + i] = sc[i] * a.scale_log2;
           }
       }
-      const uint32_t gone = (uint32_t)(missing >> ((t0 - run) >> 3)) & 0xfu;
+      const uint32_t gone = (uint32_t)(missing >> ((t0 - run) / kHalf)) & 3u;
       const bool masked = t0 + kTile > clear || gone != 0;
       if (masked) {
-        const bool bad = (gone >> g) & 1u;
-        // Of the lane's 8 keys: how many there are, and how many the row sees.
-        const int32_t here = bad ? 0 : r.length - t0 - 8 * g;
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-          const int32_t see = bad ? 0 : limit[q] - t0 - 8 * g;
+        for (int u = 0; u < 2; ++u) {
+          const bool bad = (gone >> u) & 1u;
+          const int32_t first = t0 + kHalf * u + 4 * g;
+          // Of the lane's 4 keys: how many there are, and how many the row sees.
+          const int32_t here = bad ? 0 : r.length - first;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[q][i] = i < see ? x[q][i] : -__builtin_inff();
-        }
-        // What lies behind the sequence's end may be anything: it is taken as zeros.
+          for (int q = 0; q < NQ; ++q) {
+            const int32_t see = bad ? 0 : rows.limit[q] - first;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) x[q][4 * u + i] = i < see ? x[q][4 * u + i] : -__builtin_inff();
+          }
+          // What lies behind the sequence's end may be anything: it is taken as zeros.
 #pragma unroll
-          for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w) t.vw[i][w] = i < here ? t.vw[i][w] : 0;
-          const uint32_t m = 0xffu << (8 * (i & 3));
-          t.vs[i >> 2] = i < here ? t.vs[i >> 2] : (t.vs[i >> 2] & ~m) | (0x7f7f7f7fu & m);
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w)
+              t.vw[4 * u + i][w] = i < here ? t.vw[4 * u + i][w] : 0;
+            const uint32_t m = 0xffu << (8 * i);
+            t.vs[u] = i < here ? t.vs[u] : (t.vs[u] & ~m) | (0x7f7f7f7fu & m);
+          }
         }
       }
-      if (masked && clear < most && any_nan<D, FMT>(t)) keep_nan_apart<D, FMT, NQ>(t, x, rows);
-      u32x4 vf[S::kOut];
-      decode_values<D, FMT>(t, vf);
+      if (masked && clear < most && any_nan<D, FMT>(t)) keep_nan_apart<D, FMT, NQ>(t, x, rows.state);
+      u32x4 pf[NQ][PARTS];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        softmax_step<D>(x[q], rows[q]);
-        u32x4 pf[S::kPParts];
-        split_probs<S::kPParts>(x[q], pf);
+        softmax_step<D>(x[q], rows.state[q]);
+        split_probs<PARTS>(x[q], pf[q]);
+      }
 #pragma unroll
-        for (int p = S::kPParts - 1; p >= 0; --p)
+      for (int d = 0; d < S::kOut / 2; ++d) {
+        u32x4 vf[2];
+        decode_values<D, FMT>(t, d, vf);
 #pragma unroll
-          for (int j = 0; j < S::kOut; ++j) rows[q].acc[j] = mfma(vf[j], pf[p], rows[q].acc[j]);
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              rows.state[q].acc[2 * d + e] = mfma(vf[e], pf[q][p], rows.state[q].acc[2 * d + e]);
       }
     };
     // Each step's loads are issued a step before, without a branch around them (past the run's end the last
@@ -859,154 +686,242 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT)) void mx_at
     const int32_t final = run + (run_end - 1 - run) / kTile * kTile;
     KeyTile<D, FMT> t0, t1;
     fetch(run, t0);
-    for (int32_t t = run;; t += 2 * kTile) {
+    for (int32_t t = run; t <= final; t += 2 * kTile) {
       fetch(t + kTile < final ? t + kTile : final, t1);
       use(t, t0);
-      if (t >= final) break;
       fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
-      use(t + kTile, t1);
-      if (t + kTile >= final) break;
+      if (t + kTile <= final) use(t + kTile, t1);
     }
-  }
-
-  // Waves 2, 3 hand their sums to 0, 1, then 1 to 0, in the accumulators' own layout.
-  __shared__ float buf[kWaves / 2][D / 4 + 2][64];
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-    for (int w = kWaves / 2; w >= 1; w >>= 1) {
-      if (wave >= w && wave < 2 * w) {
-#pragma unroll
-        for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) buf[wave - w][4 * j + i][lane] = rows[q].acc[j][i];
-        buf[wave - w][D / 4][lane] = rows[q].m;
-        buf[wave - w][D / 4 + 1][lane] = rows[q].l;
-      }
-      __syncthreads();
-      if (wave < w) {
-        const float mo = buf[wave][D / 4][lane];
-        const float next = __builtin_fmaxf(rows[q].m, mo);
-        const float f = __builtin_amdgcn_exp2f(rows[q].m - next), fo = __builtin_amdgcn_exp2f(mo - next);
-        rows[q].m = next;
-        rows[q].l = rows[q].l * f + buf[wave][D / 4 + 1][lane] * fo;
-#pragma unroll
-        for (int j = 0; j < S::kOut; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            rows[q].acc[j][i] = rows[q].acc[j][i] * f + buf[wave][4 * j + i][lane] * fo;
-      }
-      __syncthreads();
-    }
-  }
-  if (wave != 0) return;
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    rows[q].l = across_g(rows[q].l, true);
-    if (row_ok[q]) store_row<D, DT>(a, rows[q], orow[q], split, active > 1, g);
   }
 }
 
-// Joins the splits of one (token, head) row; rows of tiles that had one split are left alone.  D/4 lanes
-// hold the row, the workgroup's other lanes take other splits, and LDS adds them up.
+__device__ __forceinline__ RowTile uniform_rows(const AttnArgs& a, int32_t i) {
+  RowTile r = sequence_rows(a, i);
+  r.tok0 = uniform(r.tok0);
+  r.fresh = uniform(r.fresh);
+  r.rows = uniform(r.rows);
+  r.length = uniform(r.length);
+  return r;
+}
+
+// Waves of a SIMD that the step kernel's registers are held to.
+constexpr int step_occupancy(int dim, int query_tiles) { return dim == 256 || query_tiles > 1 ? 1 : 2; }
+
+template <int D, int FMT, int DT, int NQ>
+__global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
+  using S = Shape<D, FMT, DT>;
+  constexpr int kTileRows = kRows * NQ;
+  __shared__ Share found[kWaves];
+  const int32_t wave = uniform((int)threadIdx.x >> 6), worker = (int32_t)blockIdx.x * kWaves + wave;
+  const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+
+  const int32_t share = find_shares(a, kTileRows, found);
+  const int32_t h = worker % a.kv_heads;
+  int32_t at = uniform(found[wave].sequence);       // sequence, tile and step that the share begins at
+  int32_t left = uniform(found[wave].steps);
+  int32_t tile = uniform(found[wave].tile), step = uniform(found[wave].step);
+  while (left > 0) {
+    RowTile r = uniform_rows(a, at);
+    const int32_t tiles = r.rows > a.step_rows ? 0 : (r.rows + kTileRows - 1) / kTileRows;
+    if (tile >= tiles) {
+      ++at;
+      tile = step = 0;
+      continue;
+    }
+    r.row0 = tile * kTileRows;
+    const int32_t all = tile_steps(r.length);
+    const int32_t take = all - step < left ? all - step : left;
+    const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
+    const int32_t most = row_limit(a, r, last / a.group);      // keys that the tile's last row sees,
+    const int32_t clear = row_limit(a, r, r.row0 / a.group);   // and that all its rows see
+    const int32_t from = step * kTile;
+    const int32_t end = from + take * kTile < most ? from + take * kTile : most;
+    QueryRows<D, FMT, DT, NQ> rows;
+    begin_rows(a, r, h, rows);
+    attend<D, FMT, DT, NQ, S::kPParts>(a, r, h, from, end, clear, most, rows);
+
+    const bool whole = take == all;
+    const int64_t part = ((int64_t)worker * 2 + (step > 0 ? 0 : 1)) * kTileRows;
+    const int32_t pieces = 1 + (all - take + share - 1) / share;  // of the item, from its first piece
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      rows.state[q].l = across_g(rows.state[q].l, true);
+      if (!rows.ok[q]) continue;
+      if (whole)
+        store_row<D, DT>(a, rows.state[q], rows.orow[q], g);
+      else
+        store_part<D>(a, rows.state[q], part + kRows * q + n, g);
+      if (step == 0 && g == 0) {
+        a.joins[rows.orow[q] * 2] = worker;
+        a.joins[rows.orow[q] * 2 + 1] = pieces << 8 | (kRows * q + n);
+      }
+    }
+    left -= take;
+    step = 0;
+    ++tile;
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Many rows a sequence: prefill chunks.
+// ------------------------------------------------------------------------------------------
+// A workgroup takes 64 NQ consecutive rows of one kv head over all the keys they see, a wave 16 NQ of them.
+// Its waves walk the keys together, so the codes that one fetches the others find in the caches; the row
+// tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
+template <int D, int FMT, int DT, int NQ>
+__global__ __launch_bounds__(kWaves * 64, VG_CHUNK_OCC) void mx_attention_chunk_kernel(const AttnArgs a) {
+  constexpr int kTileRows = kRows * NQ, kGroupRows = kWaves * kTileRows;
+  constexpr int kParts = chunk_parts(DT);
+  const int32_t h = (int32_t)(blockIdx.x % (uint32_t)a.kv_heads);
+  const int32_t tile = (int32_t)((gridDim.x - 1 - blockIdx.x) / (uint32_t)a.kv_heads);
+  // Tiles of sequence i begin at floor(row bound / rows of a tile) + i: room for each one's last, short tile.
+  const int32_t lane = threadIdx.x & 63, g = lane >> 4;
+  int32_t i = -1;
+  for (int32_t i0 = 0; i0 < sequences(a); i0 += 64) {
+    const bool below = i0 + lane < sequences(a) && row_bound(a, i0 + lane) * a.group / kGroupRows + i0 + lane <= tile;
+    i += __popcll(__ballot(below));
+  }
+  i = uniform(i);
+  RowTile r = uniform_rows(a, i);
+  if (r.seq < 0 || r.rows <= a.step_rows) return;
+  r.row0 = (tile - (r.tok0 * a.group / kGroupRows + i)) * kGroupRows + uniform((int)threadIdx.x >> 6) * kTileRows;
+  if (r.row0 < 0 || r.row0 >= r.rows) return;
+  const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
+  const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
+  QueryRows<D, FMT, DT, NQ> rows;
+  begin_rows(a, r, h, rows);
+  attend<D, FMT, DT, NQ, kParts>(a, r, h, 0, most, clear, most, rows);
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    rows.state[q].l = across_g(rows.state[q].l, true);
+    if (!rows.ok[q]) continue;
+    store_row<D, DT>(a, rows.state[q], rows.orow[q], g);
+    if (a.joins != nullptr && g == 0) a.joins[rows.orow[q] * 2 + 1] = 1 << 8;
+  }
+}
+
+// Joins the pieces of the (token, head) rows that have several: a row's first is the last of its wave's share,
+// the others are the first of the shares that follow in the head.  D/4 lanes hold the row, the workgroup's
+// other lanes take other pieces, and LDS adds them up.
+constexpr int kMostPieces = 2048;
+
 template <int D, int DT>
-__global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a, int32_t tile_rows, int32_t rows) {
   constexpr int kLanes = D / 4, kSets = 256 / kLanes;
-  const int64_t orow = blockIdx.x;
-  const int32_t tok = (int32_t)(orow / a.q_heads), head = (int32_t)(orow - (int64_t)tok * a.q_heads);
-  RowTile r;
-  if (a.starts == nullptr) {
-    r.seq = r.tok0 = tok;
-    r.fresh = 1;
-  } else {
-    const int32_t i = find_bound(a, 1, 1, false, tok);
-    r.tok0 = row_bound(a, i);
-    r.fresh = row_bound(a, i + 1) - r.tok0;
-    r.seq = i - 1 < a.batch ? i - 1 : -1;
-  }
-  r.rows = r.fresh * a.group;
-  r.length = held_tokens(a, r.seq);
-  const int32_t row = (tok - r.tok0) * a.group + head % a.group;
-  int32_t last = row - row % a.tile_rows + a.tile_rows;
-  if (last > r.rows) last = r.rows;
-  const int32_t active = splits_of(a, row_limit(a, r, (last - 1) / a.group));
-  if (active <= 1) return;
-
-  const float* ml = a.part_ml + orow * a.splits * 2;
-  const int32_t d = threadIdx.x % kLanes, set = threadIdx.x / kLanes;
-  const float* po = a.part_o + orow * a.splits * D + 4 * d;
-  float m = -3.0e38f;
-  for (int32_t s = threadIdx.x & 63; s < active; s += 64) m = __builtin_fmaxf(m, ml[2 * s]);
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, w));
-  float l = 0.0f;
-  f32x4 o = {0, 0, 0, 0};
-  for (int32_t s = set; s < active; s += kSets) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-    l += ml[2 * s + 1] * f;
-    o += *reinterpret_cast<const f32x4*>(po + (int64_t)s * D) * f;
-  }
-  __shared__ float sums[kSets][D + 4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sums[set][4 * d + i] = o[i];
-  if (d == 0) sums[set][D] = l;
+  __shared__ float weight[kMostPieces + 1];
+  __shared__ float sums[kSets][D];
+  __shared__ float wave_top[4], wave_sum[4];
+  __shared__ int32_t found[256];
+  __shared__ int32_t count;
+  const int32_t tid = threadIdx.x, d = tid % kLanes, set = tid / kLanes;
+  const int64_t all = (int64_t)a.q_tokens * a.q_heads, row0 = (int64_t)blockIdx.x * rows;
+  if (tid == 0) count = 0;
   __syncthreads();
-  const int32_t e = threadIdx.x;
-  if (e >= D) return;
-  float total = 0.0f, x = 0.0f;
+  if (tid < rows && row0 + tid < all && (a.joins[(row0 + tid) * 2 + 1] >> 8) > 1) found[atomicAdd(&count, 1)] = tid;
+  __syncthreads();
+  for (int32_t k = 0; k < count; ++k) {
+    const int64_t orow = row0 + found[k];
+    const int32_t first = a.joins[orow * 2], packed = a.joins[orow * 2 + 1];
+    const int32_t active = packed >> 8;
+    auto place = [&](int32_t s) {
+      return ((int64_t)(first + s * a.kv_heads) * 2 + (s == 0 ? 1 : 0)) * tile_rows + (packed & 0xff);
+    };
+    float m = -3.0e38f;
+    for (int32_t s = tid; s < active; s += 256) m = __builtin_fmaxf(m, a.part_ml[place(s) * 2]);
 #pragma unroll
-  for (int i = 0; i < kSets; ++i) {
-    total += sums[i][D];
-    x += sums[i][e];
+    for (int w = 1; w < 64; w <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, w));
+    if ((tid & 63) == 0) wave_top[tid >> 6] = m;
+    __syncthreads();
+    m = __builtin_fmaxf(__builtin_fmaxf(wave_top[0], wave_top[1]), __builtin_fmaxf(wave_top[2], wave_top[3]));
+    float l = 0.0f;
+    for (int32_t s = tid; s < active; s += 256) {
+      const float f = __builtin_amdgcn_exp2f(a.part_ml[place(s) * 2] - m);
+      weight[s] = f;
+      l += a.part_ml[place(s) * 2 + 1] * f;
+    }
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) l += __shfl_xor(l, w);
+    if ((tid & 63) == 0) wave_sum[tid >> 6] = l;
+    __syncthreads();
+    l = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int32_t s = set; s < active; s += kSets)
+      o += *reinterpret_cast<const f32x4*>(a.part_o + place(s) * D + 4 * d) * weight[s];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[set][4 * d + i] = o[i];
+    __syncthreads();
+    if (tid < D) {
+      float x = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) x += sums[i][tid];
+      const bool empty = l == 0.0f;
+      Codec<DT>::store1(a.out, orow * D + tid, empty ? 0.0f : x / l);
+      if (a.lse != nullptr && tid == 0)
+        a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(l)) * 0.693147180559945309f;
+    }
+    __syncthreads();
   }
-  const bool empty = total == 0.0f;
-  Codec<DT>::store1(a.out, orow * D + e, empty ? 0.0f : x / total);
-  if (a.lse != nullptr && e == 0)
-    a.lse[orow] = empty ? -__builtin_inff() : (m + log2f(total)) * 0.693147180559945309f;
 }
 
-// How a call is laid out: workgroups over row tiles, heads and splits of the keys.
+// How a call is laid out.
 struct AttnPlan {
-  int64_t row_tiles;
-  int32_t tile_rows;
-  int32_t query_tiles;  // of 16 rows a wave, in the kernel for few rows; 0: the kernel for many
-  int32_t chunk, splits;
+  int32_t query_tiles;  // of a wave of the step kernel: 1, 2 or 4
+  int32_t workers;      // its waves
+  int32_t least_steps;
+  int32_t step_rows;    // sequences of more rows go to the chunk kernel
+  int64_t chunk_tiles;  // its workgroups for each kv head; 0: not launched
+  bool steps;           // whether the step kernel is launched
 };
 
-AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, bool ragged,
-                        int64_t most, int cus) {
+AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                        int32_t dtype, bool ragged, int cus) {
   AttnPlan p;
-  const int64_t group = q_heads / kv_heads;
+  const int64_t group = q_heads / kv_heads, tiles = most_tiles((int)head_dim, dtype);
+  const int64_t chunk_rows = kWaves * kRows * tiles;
+  p.steps = true;
+  p.chunk_tiles = 0;
+  p.step_rows = INT32_MAX;
+  // Chunks where their workgroups fill the card; the step kernel splits the keys where they do not.
+  if (ragged && q_tokens * q_heads >= chunk_rows * cus) {
+    p.chunk_tiles = q_tokens * group / chunk_rows + batch + 2;
+    p.step_rows = kRows * 4;
+  }
   // Rows of a sequence, on average.
   const int64_t rows = ragged ? q_tokens * group / (batch > 0 ? batch : 1) : group;
-  p.query_tiles = rows <= 64 ? 1 : 0;
-  p.tile_rows = p.query_tiles > 0 ? kRows * p.query_tiles : kWaves * kRows;
-  p.row_tiles = ragged ? q_tokens * group / p.tile_rows + batch + 2
-                       : batch * ((group + p.tile_rows - 1) / p.tile_rows);
-  // Splits of the keys, so that there are about eight workgroups for each CU: sequences differ in length, and
-  // many short workgroups even that out.
-  const int64_t base = p.row_tiles * kv_heads;
-  const int64_t want = (kStepGroups * (int64_t)cus + base - 1) / base;
-  int64_t chunk = (most + want - 1) / want;
-  chunk = (chunk + kWaves * kTile - 1) / (kWaves * kTile) * (kWaves * kTile);
-  const int64_t least = kWaves * kTile * 2;
-  if (chunk < least) chunk = least;
-  p.chunk = (int32_t)chunk;
-  p.splits = (int32_t)((most + chunk - 1) / chunk);
-  if (p.splits < 1) p.splits = 1;
+  p.query_tiles = p.chunk_tiles > 0 || rows <= kRows || tiles < 2 ? 1 : rows <= 2 * kRows || tiles < 4 ? 2 : 4;
+  // As many waves as the card holds at once: every one runs from the start, with an equal share.
+  p.workers = cus * step_occupancy((int)head_dim, p.query_tiles) * kWaves;
+  if (p.workers > kMostPieces) p.workers = kMostPieces;
+  // At least one share for each head.
+  if (p.workers < kv_heads) p.workers = (int32_t)((kv_heads + kWaves - 1) / kWaves * kWaves);
+  p.least_steps = kLeastSteps;
   return p;
+}
+
+size_t workspace_bytes(const AttnPlan& p, int64_t q_tokens, int64_t q_heads, int64_t head_dim) {
+  return (size_t)p.workers * 2 * kRows * (size_t)p.query_tiles * (size_t)(head_dim + 2) * sizeof(float) +
+         (size_t)q_tokens * (size_t)q_heads * 2 * sizeof(int32_t);
 }
 
 template <int D, int FMT, int DT>
 void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-  const dim3 grid((uint32_t)(a.kv_heads * p.row_tiles * a.splits));
-  if (p.query_tiles == 1)
-    hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 1>), grid, dim3(kWaves * 64), 0, st, a);
-  else
-    hipLaunchKernelGGL((mx_attention_kernel<D, FMT, DT>), grid, dim3(kWaves * 64), 0, st, a);
-  if (a.splits > 1)
-    hipLaunchKernelGGL((mx_attention_join_kernel<D, DT>), dim3((uint32_t)a.q_tokens * (uint32_t)a.q_heads),
-                       dim3(256), 0, st, a);
+  constexpr int kMost = most_tiles(D, DT);
+  const dim3 block(kWaves * 64), steps((uint32_t)p.workers / kWaves);
+  if (p.chunk_tiles > 0)
+    hipLaunchKernelGGL((mx_attention_chunk_kernel<D, FMT, DT, kMost>),
+                       dim3((uint32_t)(p.chunk_tiles * a.kv_heads)), block, 0, st, a);
+  if (p.query_tiles == 4) {
+    if constexpr (kMost >= 4) hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 4>), steps, block, 0, st, a);
+  } else if (p.query_tiles == 2) {
+    if constexpr (kMost >= 2) hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 2>), steps, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 1>), steps, block, 0, st, a);
+  }
+  const int64_t all = (int64_t)a.q_tokens * a.q_heads;
+  const int64_t rows = all <= 4096 ? 1 : all <= 16 * 4096 ? 16 : 256;
+  hipLaunchKernelGGL((mx_attention_join_kernel<D, DT>), dim3((uint32_t)((all + rows - 1) / rows)), dim3(256), 0, st,
+                     a, kRows * p.query_tiles, (int32_t)rows);
 }
 
 template <int FMT, int DT>
@@ -1050,22 +965,19 @@ int32_t check_attention(const char* what, int64_t q_tokens, int64_t batch, int64
 
 extern "C" {
 
-VELOGRAD_API size_t velograd_mx_cache_attention_workspace_bytes(int64_t q_tokens, int64_t sequences,
-                                                                int64_t q_heads, int64_t kv_heads,
-                                                                int64_t head_dim, int64_t table_width,
-                                                                int64_t page_size, int32_t ragged,
-                                                                int32_t device) {
+VELOGRAD_API size_t velograd_mx_cache_attention_workspace_bytes(
+    int64_t q_tokens, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+    int64_t table_width, int64_t page_size, int32_t ragged, int32_t dtype, int32_t mx_format, int32_t device) {
   const char* what = "velograd_mx_cache_attention_workspace_bytes";
-  if (check_mx_cache(what, kv_heads, head_dim, 0, page_size, VELOGRAD_MX_E2M1) != 0 ||
+  if (elem_bytes_of(dtype) == 0 || check_mx_cache(what, kv_heads, head_dim, 0, page_size, mx_format) != 0 ||
       check_attention(what, q_tokens, sequences, q_heads, kv_heads, head_dim, table_width, page_size,
                       ragged != 0) != 0)
     return 0;
   const int cus = cu_count(device);
   if (cus <= 0 || q_tokens == 0) return 0;
-  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, ragged != 0,
-                                    table_width * page_size, cus);
-  if (p.splits <= 1) return 0;
-  return (size_t)q_tokens * (size_t)q_heads * (size_t)p.splits * (size_t)(head_dim + 2) * sizeof(float);
+  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, dtype,
+                                    ragged != 0, cus);
+  return workspace_bytes(p, q_tokens, q_heads, head_dim);
 }
 
 VELOGRAD_API int32_t velograd_mx_cache_attention(
@@ -1104,15 +1016,15 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
     return fail(VELOGRAD_ERR_DEVICE_QUERY, "%s: hipGetDevice failed", what);
   const int cus = cu_count(device);
   if (cus <= 0) return fail(VELOGRAD_ERR_DEVICE_QUERY, "%s: cannot query device %d", what, device);
-  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, ragged,
-                                    pages > 0 ? table_width * page_size : 0, cus);
-  const size_t rows = (size_t)q_tokens * (size_t)q_heads * (size_t)p.splits;
-  if (p.splits > 1 && (workspace == nullptr || ws_bytes < rows * (size_t)(head_dim + 2) * sizeof(float)))
-    return fail(VELOGRAD_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes,
-                rows * (size_t)(head_dim + 2) * sizeof(float));
-  if (p.row_tiles > INT32_MAX / p.splits || p.row_tiles * p.splits > INT32_MAX / kv_heads)
+  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, dtype, ragged, cus);
+  if (p.chunk_tiles > INT32_MAX / kv_heads)
     return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: %lld row tiles exceed the grid limit", what,
-                (long long)p.row_tiles);
+                (long long)p.chunk_tiles);
+  const size_t need = workspace_bytes(p, q_tokens, q_heads, head_dim);
+  if (workspace == nullptr || ws_bytes < need)
+    return fail(VELOGRAD_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
+  if (!aligned16(workspace))
+    return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
 
   AttnArgs a;
   a.q = q;
@@ -1126,7 +1038,9 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   a.out = out;
   a.lse = lse;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o == nullptr ? nullptr : a.part_o + rows * (size_t)head_dim;
+  const size_t part_rows = (size_t)p.workers * 2 * kRows * (size_t)p.query_tiles;
+  a.part_ml = a.part_o + part_rows * (size_t)head_dim;
+  a.joins = reinterpret_cast<int32_t*>(a.part_ml + part_rows * 2);
   a.q_t = q_token_stride;
   a.q_h = q_head_stride;
   a.table_stride = table_stride;
@@ -1140,10 +1054,9 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   a.page_shift = 0;
   while (((int64_t)1 << a.page_shift) < page_size) ++a.page_shift;
   a.causal = causal != 0 ? 1 : 0;
-  a.row_tiles = (int32_t)p.row_tiles;
-  a.tile_rows = p.tile_rows;
-  a.chunk = p.chunk;
-  a.splits = p.splits;
+  a.workers = p.workers;
+  a.least_steps = p.least_steps;
+  a.step_rows = p.step_rows;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634074);
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   switch (dtype) {

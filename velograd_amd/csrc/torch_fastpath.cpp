@@ -402,7 +402,7 @@ Tensors mx_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor
   if (starts.has_value() ? !mx_index(*starts, at::kInt, sequences + 1) : tokens != sequences) return {};
   const size_t bytes = velograd_mx_cache_attention_workspace_bytes(
       tokens, sequences, heads, s.kv_heads, s.head_dim, table.size(1), s.page_size,
-      starts.has_value() ? 1 : 0, q.get_device());
+      starts.has_value() ? 1 : 0, code, s.format, q.get_device());
   at::Tensor out = at::empty(q.sizes(), q.options()), lse, ws;
   if (want_lse) lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
   if (bytes != 0) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));

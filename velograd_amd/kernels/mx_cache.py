@@ -338,7 +338,7 @@ def mx_cache_attention(q: torch.Tensor, cache: MXCache, block_table: torch.Tenso
         index = device.index if device.index is not None else torch.cuda.current_device()
         size = lib.velograd_mx_cache_attention_workspace_bytes(
             tokens, sequences, heads, shape.kv_heads, shape.head_dim, block_table.shape[1],
-            shape.page_size, 0 if q_starts is None else 1, index)
+            shape.page_size, 0 if q_starts is None else 1, code, shape.fmt, index)
         ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         rc = lib.velograd_mx_cache_attention(
             q.data_ptr(), *(t.data_ptr() for t in cache), block_table.data_ptr(), lengths.data_ptr(),
