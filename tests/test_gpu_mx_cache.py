@@ -16,6 +16,8 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 # each off by at most 2^-8 of what the parts before leave; two for 2-byte outputs, three for float32.
 OUT_EPS = {t: torch.finfo(t).eps / 2 for t in DTYPES.values()}
 P_EPS = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -16, torch.float32: 2.0 ** -24}
+# Of chunks: one part for bf16.
+CHUNK_P_EPS = {**P_EPS, torch.bfloat16: 2.0 ** -8}
 
 
 @pytest.fixture(autouse=True, params=["fast path", "general path"])
@@ -205,12 +207,12 @@ def _attend(q, parts, table, lengths, starts, fmt, **kw):
     return vk.mx_cache_attention(q, cache, t, ln, st, return_lse=True, **kw)
 
 
-def _check(got, q, parts, table, lengths, starts, page, fmt, scale=None, causal=True):
+def _check(got, q, parts, table, lengths, starts, page, fmt, scale=None, causal=True, p_eps=None):
     out, lse = got
     dim = q.shape[-1]
     scale = dim ** -0.5 if scale is None else scale
     want, wlse, off, lse_off = R.attention(q.double().cpu().numpy(), parts, table, lengths, starts, page, fmt,
-                                           scale, causal, OUT_EPS[q.dtype], P_EPS[q.dtype])
+                                           scale, causal, OUT_EPS[q.dtype], P_EPS[q.dtype] if p_eps is None else p_eps)
     assert out.dtype == q.dtype and out.shape == q.shape and lse.dtype == torch.float32
     o, s = out.double().cpu().numpy(), lse.double().cpu().numpy()
     empty = np.isneginf(wlse)
@@ -258,6 +260,49 @@ def test_attention(dtype, fmt, dim, heads, kv, page, lengths, fresh, pad, causal
     # the same call gives the same bits
     again = _attend(q, parts, table, lengths, starts, fmt, causal=causal)
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+CHUNKS = [
+    # enough rows for the kernel that takes 64 rows of a sequence a wave, others and padding beside them:
+    # dtype, fmt, dim, heads, kv heads, page, lengths, new tokens, padding rows
+    ("bf16", "e2m1", 64, 32, 8, 16, [2100], [2060], 0),
+    ("bf16", "e2m1", 128, 16, 2, 64, [1500, 40, 0, 3000, 333], [1500, 1, 3, 2400, 250], 70),
+    ("bf16", "e4m3", 256, 24, 3, 32, [1400], [1399], 1),
+    ("fp16", "e2m1", 128, 30, 6, 16, [1300, 17], [1280, 2], 300),
+    ("fp32", "e4m3", 64, 40, 8, 128, [900, 10], [880, 20], 0),
+    ("fp32", "e2m1", 128, 32, 32, 16, [600, 700], [500, 600], 3),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,fmt,dim,heads,kv,page,lengths,fresh,pad", CHUNKS)
+def test_attention_of_chunks(dtype, fmt, dim, heads, kv, page, lengths, fresh, pad, causal):
+    _say(f"chunks {dtype} {fmt} dim {dim} {heads}/{kv} page {page} {lengths} {fresh} pad {pad} causal {causal}")
+    rng = np.random.default_rng(sum(lengths) + dim)
+    parts, table, starts, q = _setup(rng, DTYPES[dtype], fmt, dim, heads, kv, page, lengths, fresh, pad)
+    got = _attend(q, parts, table, lengths, starts, fmt, causal=causal)
+    _check(got, q, parts, table, lengths, starts, page, fmt, causal=causal, p_eps=CHUNK_P_EPS[DTYPES[dtype]])
+    again = _attend(q, parts, table, lengths, starts, fmt, causal=causal)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+def test_chunks_keep_nan_values_from_rows_that_do_not_see_them():
+    _say("chunks NaN")
+    rng = np.random.default_rng(17)
+    parts, table, starts, q = _setup(rng, torch.bfloat16, "e2m1", 64, 32, 1, 16, [2200], [2100], 0)
+    clean = _attend(q, parts, table, [2200], starts, "e2m1")
+    for t in (50, 1000):
+        parts[3][table[0, t // 16], 0, 1, t % 16] = 255          # dims 32..63
+    out, lse = _attend(q, parts, table, [2200], starts, "e2m1")
+    assert torch.isnan(out[..., 32:]).all()                       # every row sees key 50
+    assert torch.equal(out[..., :32], clean[0][..., :32]) and torch.equal(lse, clean[1])
+    parts[3][table[0, 50 // 16], 0, 1, 50 % 16] = 127
+    parts[2][table[0, 50 // 16], 0, 50 % 16] = 0
+    clean = _attend(q, parts, table, [2200], starts, "e2m1")
+    out, lse = _attend(q, parts, table, [2200], starts, "e2m1")
+    first = 1000 - 100                                            # row i sees keys up to 100 + i
+    assert torch.isnan(out[first:, :, 32:]).all() and not torch.isnan(out[:first]).any()
+    assert torch.equal(out[..., :32], clean[0][..., :32])
 
 
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])

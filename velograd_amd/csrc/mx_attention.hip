@@ -456,9 +456,14 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, int32_t
   using S = Shape<D, FMT, DT>;
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
+    const int64_t at = e + (4 * (8 * s / S::kChunkElems) + g) * S::kChunkElems + 8 * s % S::kChunkElems;
+    if constexpr (S::kQParts == 1) {
+      qf[s][0] = u32x4{0u, 0u, 0u, 0u};
+      if (ok) qf[s][0] = load16_any<DT>(a.q, at);
+      continue;
+    }
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (ok) {
-      const int64_t at = e + (4 * (8 * s / S::kChunkElems) + g) * S::kChunkElems + 8 * s % S::kChunkElems;
       Codec<DT>::unpack(load16_any<DT>(a.q, at), f);
       if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, at + 4), f + 4);
     }
@@ -478,79 +483,84 @@ __device__ __forceinline__ int64_t take_lane(int64_t v, int32_t lane) {
 // Steps of an item: a tile of rows of one kv head over everything its sequence holds.
 __device__ inline int32_t tile_steps(int32_t length) { return length <= kTile ? 1 : (length + kTile - 1) / kTile; }
 
+// Row tiles of a sequence in the step kernel; rows of no sequence are all its own.
+__device__ __forceinline__ int32_t row_tiles(const AttnArgs& a, const RowTile& r, int32_t tile_rows) {
+  return r.seq >= 0 && r.rows > a.step_rows ? 0 : (r.rows + tile_rows - 1) / tile_rows;
+}
+
+__device__ __forceinline__ int32_t sequence_steps(const AttnArgs& a, const RowTile& r, int32_t tile_rows) {
+  return row_tiles(a, r, tile_rows) * tile_steps(r.length);
+}
+
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ int32_t wave_scan(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, :2, :4, :8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
+__device__ __forceinline__ RowTile sequence_rows_or_none(const AttnArgs& a, int32_t i) {
+  if (i < sequences(a)) return sequence_rows(a, i);
+  return RowTile{-1, 0, 0, 0, 0, 0};
+}
+
 // A wave's share of a head's steps, in the order sequence, row tile, step.
 struct Share {
-  int32_t sequence, tile, step;        // where it begins
-  int32_t steps;                       // how many it has
+  int32_t sequence, tile, step;  // where it begins
+  int32_t steps;                 // how many it has; 0: none
+  int32_t each;                  // how many every share but the last has
+  RowTile rows;                  // of the sequence
 };
-
-__device__ inline int64_t sequence_steps(const AttnArgs& a, int32_t i, int32_t tile_rows) {
-  if (i >= sequences(a)) return 0;
-  const RowTile r = sequence_rows(a, i);
-  if (r.rows > a.step_rows) return 0;
-  return (int64_t)((r.rows + tile_rows - 1) / tile_rows) * tile_steps(r.length);
-}
 
 // Sequences differ in length, so a head's steps are dealt out in equal shares of consecutive ones, each to one
 // wave, whatever items they belong to; wave w takes head w % kv_heads, so neighbouring waves read the same
-// pages.  Every workgroup adds up all sequences' steps, and finds the sequences that its waves' shares begin
-// in.  Returns the steps of every share but the last.
-__device__ inline int32_t find_shares(const AttnArgs& a, int32_t tile_rows, Share* found) {
-  __shared__ int64_t sums[2][kWaves];
-  const int32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = kWaves * 64;
-  const int32_t count = sequences(a);
-  if (tid < kWaves) found[tid].steps = 0;
-  const int64_t mine = sequence_steps(a, tid, tile_rows);
-  int64_t total = mine;
-  for (int32_t i = tid + threads; i < count; i += threads) total += sequence_steps(a, i, tile_rows);
-#pragma unroll
-  for (int w = 1; w < 64; w <<= 1) total += __shfl_xor(total, w);
-  if (lane == 0) sums[0][wave] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) total += sums[0][w];
-  const int32_t each = a.workers / a.kv_heads;  // shares of a head
-  int64_t share = (total + each - 1) / each;
-  if (share < a.least_steps) share = a.least_steps;
-  const int32_t worker = (int32_t)blockIdx.x * kWaves;
-  const int64_t begin = share * (worker / a.kv_heads), ending = share * ((worker + kWaves - 1) / a.kv_heads);
-  int64_t before = 0;  // steps before the sequences at hand
-  for (int32_t i0 = 0; i0 < count; i0 += threads) {
-    const int64_t one = i0 == 0 ? mine : sequence_steps(a, i0 + tid, tile_rows);
-    int64_t upto = one;  // inclusive, within the wave
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      const int64_t x = __shfl_up(upto, w);
-      if (lane >= w) upto += x;
-    }
-    if (i0 > 0) __syncthreads();
-    if (lane == 63) sums[1][wave] = upto;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) upto += sums[1][w];
-      all += sums[1][w];
-    }
-    const int64_t lo = before + upto - one, hi = before + upto;
-    if (hi > begin && lo <= ending && one > 0) {
-      const int32_t steps = tile_steps(held_tokens(a, a.starts == nullptr ? i0 + tid : i0 + tid - 1));
-#pragma unroll 1
-      for (int w = 0; w < kWaves; ++w) {
-        const int64_t from = share * ((worker + w) / a.kv_heads);
-        if (from < lo || from >= hi) continue;
-        found[w].sequence = i0 + tid;
-        found[w].tile = (int32_t)((from - lo) / steps);
-        found[w].step = (int32_t)(from - lo - (int64_t)found[w].tile * steps);
-        found[w].steps = (int32_t)(total - from < share ? total - from : share);
-      }
-    }
-    before += all;
-    if (before > ending) break;
+// pages.  Every wave adds up all sequences' steps, 64 at a time, and finds the one that its share begins in.
+__device__ __forceinline__ Share find_share(const AttnArgs& a, int32_t tile_rows, int32_t worker) {
+  const int32_t lane = threadIdx.x & 63, count = sequences(a);
+  RowTile r = sequence_rows_or_none(a, lane);
+  int32_t mine = sequence_steps(a, r, tile_rows);
+  int32_t upto = wave_scan(mine);
+  int32_t total = __builtin_amdgcn_readlane(upto, 63);
+  if (count > 64) {
+    int32_t more = 0;
+    for (int32_t i = lane + 64; i < count; i += 64) more += sequence_steps(a, sequence_rows(a, i), tile_rows);
+    total += __builtin_amdgcn_readlane(wave_scan(more), 63);
   }
-  __syncthreads();
-  return uniform((int32_t)share);
+  const int32_t shares = a.workers / a.kv_heads;  // of a head
+  Share s;
+  s.each = (int32_t)(((uint32_t)total + (uint32_t)shares - 1) / (uint32_t)shares);
+  if (s.each < a.least_steps) s.each = a.least_steps;
+  const int64_t from = (int64_t)s.each * (worker / a.kv_heads);
+  s.steps = 0;
+  if (from >= total) return s;
+  s.steps = total - (int32_t)from < s.each ? total - (int32_t)from : s.each;
+  int32_t before = 0;
+  for (int32_t i0 = 0;; i0 += 64) {
+    if (i0 > 0) {
+      r = sequence_rows_or_none(a, i0 + lane);
+      mine = sequence_steps(a, r, tile_rows);
+      upto = wave_scan(mine);
+    }
+    const uint64_t here = __ballot((int32_t)from < before + upto);
+    if (here != 0) {
+      const int32_t l = __builtin_ctzll(here);  // the first sequence whose steps reach past `from`
+      const int32_t in = (int32_t)from - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
+      s.sequence = i0 + l;
+      s.rows.seq = a.starts == nullptr ? s.sequence : s.sequence - 1 < a.batch ? s.sequence - 1 : -1;
+      s.rows.tok0 = __builtin_amdgcn_readlane(r.tok0, l);
+      s.rows.fresh = __builtin_amdgcn_readlane(r.fresh, l);
+      s.rows.rows = __builtin_amdgcn_readlane(r.rows, l);
+      s.rows.length = __builtin_amdgcn_readlane(r.length, l);
+      s.tile = (int32_t)((uint32_t)in / (uint32_t)tile_steps(s.rows.length));
+      s.step = in - s.tile * tile_steps(s.rows.length);
+      return s;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
 }
 
 // A wave's query rows: 16 NQ rows of a tile, each in a lane's column.
@@ -711,20 +721,16 @@ template <int D, int FMT, int DT, int NQ>
 __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
   using S = Shape<D, FMT, DT>;
   constexpr int kTileRows = kRows * NQ;
-  __shared__ Share found[kWaves];
-  const int32_t wave = uniform((int)threadIdx.x >> 6), worker = (int32_t)blockIdx.x * kWaves + wave;
+  const int32_t worker = (int32_t)blockIdx.x * kWaves + uniform((int)threadIdx.x >> 6);
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 
-  const int32_t share = find_shares(a, kTileRows, found);
+  const Share share = find_share(a, kTileRows, worker);
   const int32_t h = worker % a.kv_heads;
-  int32_t at = uniform(found[wave].sequence);       // sequence, tile and step that the share begins at
-  int32_t left = uniform(found[wave].steps);
-  int32_t tile = uniform(found[wave].tile), step = uniform(found[wave].step);
+  int32_t at = share.sequence, tile = share.tile, step = share.step, left = share.steps;
+  RowTile r = share.rows;
   while (left > 0) {
-    RowTile r = uniform_rows(a, at);
-    const int32_t tiles = r.rows > a.step_rows ? 0 : (r.rows + kTileRows - 1) / kTileRows;
-    if (tile >= tiles) {
-      ++at;
+    if (tile >= row_tiles(a, r, kTileRows)) {
+      r = uniform_rows(a, ++at);
       tile = step = 0;
       continue;
     }
@@ -742,7 +748,7 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
 
     const bool whole = take == all;
     const int64_t part = ((int64_t)worker * 2 + (step > 0 ? 0 : 1)) * kTileRows;
-    const int32_t pieces = 1 + (all - take + share - 1) / share;  // of the item, from its first piece
+    const int32_t pieces = 1 + (all - take + share.each - 1) / share.each;  // of the item, from its first piece
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       rows.state[q].l = across_g(rows.state[q].l, true);
@@ -1017,6 +1023,13 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   const int cus = cu_count(device);
   if (cus <= 0) return fail(VELOGRAD_ERR_DEVICE_QUERY, "%s: cannot query device %d", what, device);
   const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, dtype, ragged, cus);
+  // The waves count steps in 32 bits: those of the sequences that the step kernel takes.
+  const int64_t step_tiles = p.chunk_tiles > 0 ? sequences * ((p.step_rows + kRows - 1) / kRows)
+                                               : q_tokens * (q_heads / kv_heads) / kRows + sequences;
+  const int64_t most_steps = table_width * page_size / kTile + 1;
+  if (step_tiles + q_tokens * (q_heads / kv_heads) / kRows + 2 > INT32_MAX / most_steps)
+    return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: %lld tokens over %lld pages are too many", what,
+                (long long)q_tokens, (long long)table_width);
   if (p.chunk_tiles > INT32_MAX / kv_heads)
     return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: %lld row tiles exceed the grid limit", what,
                 (long long)p.chunk_tiles);
