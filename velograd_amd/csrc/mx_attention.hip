@@ -73,7 +73,8 @@ struct AttnArgs {
   int32_t workers;         // waves of the step kernel
   int32_t least_steps;     // its smallest share
   int32_t step_rows;       // sequences of more rows are the chunk kernel's
-  float scale_log2;        // scale * log2(e)
+  float scale_log2;        // |scale| * log2(e), or 1
+  float q_factor;          // what queries are multiplied by: the scale's sign, or 0
 };
 
 // The rows that one workgroup takes: rows row0 .. of the `rows` = new * group (token, head) pairs of
@@ -156,7 +157,9 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 x, const u32x4 y, const f32x4 
 
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
   const bf16x2 p = {(__bf16)x, (__bf16)y};
-  return __builtin_bit_cast(uint32_t, p);
+  uint32_t w = __builtin_bit_cast(uint32_t, p);
+  asm("" : "+v"(w));  // one conversion: the halves that are taken out of w again are not converted anew
+  return w;
 }
 
 // f[8] as PARTS bf16 fragments whose sum is f (to 8 PARTS bits); the rest goes back into f.  A value that
@@ -279,6 +282,93 @@ __device__ __forceinline__ void load_half(const AttnArgs& a, const LaneView& c, 
   t.vs[u] = *reinterpret_cast<const uint32_t*>(vq + c.vs);
 }
 
+// The same tile by way of LDS: copied there without passing registers, 16 bytes a lane from whole lines (past
+// the caches that nothing else reads it from), kStages - 1 tiles ahead, into a ring of the wave's own.
+template <int D, int FMT>
+struct Stage {
+  using S = typename KeyTile<D, FMT>::S;
+  static constexpr int kHalfBytes = kHalf * S::kRowBytes;       // codes of a half's keys, or values
+  static constexpr int kScaleWords = D / 2;                     // of both, [keys or values][half][block][key / 4]
+  static constexpr int kScaleLoads = (kScaleWords + 63) / 64;
+  static constexpr int kCodes = 4 * kHalfBytes;                 // keys, then values, each half by half
+  static constexpr int kBytes = kCodes + 256 * kScaleLoads;
+  static constexpr int kCodeLoads = kCodes / 1024;
+  static constexpr int kLoads = kCodeLoads + kScaleLoads;
+};
+
+typedef __attribute__((address_space(3))) void LdsVoid;
+typedef const __attribute__((address_space(1))) void GlobalVoid;
+
+// An address that is the same for the wave, kept in scalar registers: the loads add the lane's own 32 bits.
+typedef const __attribute__((address_space(1))) uint8_t GlobalByte;
+__device__ __forceinline__ GlobalByte* scalar(const uint8_t* p) {
+  GlobalByte* q = (GlobalByte*)p;
+  asm("" : "+s"(q));
+  return q;
+}
+
+// To lane l's 16 (or 4) bytes behind `to`; the last argument marks the data as not to be kept (nt).
+__device__ __forceinline__ void copy16_to_lds(GlobalByte* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((GlobalVoid*)from, (LdsVoid*)to, 16, 0, 2);
+}
+__device__ __forceinline__ void copy4_to_lds(GlobalByte* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((GlobalVoid*)from, (LdsVoid*)to, 4, 0, 2);
+}
+
+// Lets at most N loads stay in flight, in order, and LDS reads none.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "the counter has 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+  asm volatile("" ::: "memory");
+}
+
+template <int D, int FMT>
+__device__ __forceinline__ void stage_tile(const AttnArgs& a, int64_t code0, int64_t code1, int64_t scale0,
+                                           int64_t scale1, uint8_t* to) {
+  using T = Stage<D, FMT>;
+  const int32_t lane = threadIdx.x & 63;
+  if constexpr (T::kHalfBytes >= 1024) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < T::kHalfBytes / 1024; ++i) {
+        const uint32_t at = 16 * lane;
+        copy16_to_lds(scalar(a.kc + (u == 0 ? code0 : code1) + 1024 * i) + at, to + u * T::kHalfBytes + 1024 * i);
+        copy16_to_lds(scalar(a.vc + (u == 0 ? code0 : code1) + 1024 * i) + at, to + (2 + u) * T::kHalfBytes + 1024 * i);
+      }
+  } else {  // 512 bytes: both halves in one
+    const int64_t at = (lane < 32 ? code0 : code1) + 16 * (lane & 31);
+    copy16_to_lds((GlobalByte*)a.kc + at, to);
+    copy16_to_lds((GlobalByte*)a.vc + at, to + 2 * T::kHalfBytes);
+  }
+#pragma unroll
+  for (int i = 0; i < T::kScaleLoads; ++i) {
+    const int32_t w = (64 * i + lane) % T::kScaleWords;  // lanes past the last word load it again
+    const int64_t at = (w / (D / 8) & 1 ? scale1 : scale0) + (((w / 4) % (D / 32)) << a.page_shift) + 4 * (w & 3);
+    copy4_to_lds((GlobalByte*)(w < D / 4 ? a.ks : a.vs) + at, to + T::kCodes + 256 * i);
+  }
+}
+
+template <int D, int FMT>
+__device__ __forceinline__ void read_stage(const uint8_t* from, int32_t n, int32_t g, KeyTile<D, FMT>& t) {
+  using S = typename KeyTile<D, FMT>::S;
+  using T = Stage<D, FMT>;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+#pragma unroll
+    for (int i = 0; i < S::kChunks; ++i) {
+      load_words<S::kChunkBytes>(from + u * T::kHalfBytes + n * S::kRowBytes + (4 * i + g) * S::kChunkBytes,
+                                 t.kw[u] + i * (S::kChunkBytes / 4));
+      t.ks[u][i] = from[T::kCodes + (u * (D / 32) + ((4 * i + g) * S::kChunkElems) / 32) * kHalf + n];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      load_words<S::kVBytes>(from + (2 + u) * T::kHalfBytes + (4 * g + i) * S::kRowBytes + n * S::kVBytes, t.vw[4 * u + i]);
+    t.vs[u] = *reinterpret_cast<const uint32_t*>(from + T::kCodes + ((2 + u) * (D / 32) + (n * (D / 16)) / 32) * kHalf + 4 * g);
+  }
+}
+
 // K of the tile: fragment s of half u holds elements 8 s .. 8 s + 7 of the lane's part of key n.
 template <int D, int FMT>
 __device__ __forceinline__ void decode_keys(const KeyTile<D, FMT>& t, u32x4 (*kf)[D / 32]) {
@@ -322,11 +412,11 @@ struct RowState {
   float m, l;
 };
 
-// x becomes the probabilities' exponents' arguments less the maximum; updates m, l, acc.
+// Scores x become probabilities; updates m, l, acc.  `c` > 0 is the scale times log2(e).
 template <int D>
-__device__ __forceinline__ void softmax_step(float* x, RowState<D>& r) {
+__device__ __forceinline__ void softmax_step(float* x, float c, RowState<D>& r) {
   float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
-                              __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7])));
+                              __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7]))) * c;
   // The running maximum moves only when a row's new maximum passes it by 8 (p stays below 2^8, which
   // costs fp32 nothing): most steps rescale nothing.
   if (__ballot(top > r.m + 8.0f) != 0) {
@@ -339,7 +429,7 @@ __device__ __forceinline__ void softmax_step(float* x, RowState<D>& r) {
     for (int j = 0; j < D / 16; ++j) r.acc[j] *= f;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - r.m);
+  for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -r.m));
   r.l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 }
 
@@ -460,6 +550,13 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, int32_t
     if constexpr (S::kQParts == 1) {
       qf[s][0] = u32x4{0u, 0u, 0u, 0u};
       if (ok) qf[s][0] = load16_any<DT>(a.q, at);
+      if (a.q_factor != 1.0f) {
+        float f[8];
+        Codec<DT>::unpack(qf[s][0], f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= a.q_factor;
+        qf[s][0] = Codec<DT>::pack(f);
+      }
       continue;
     }
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -467,6 +564,8 @@ __device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, int32_t
       Codec<DT>::unpack(load16_any<DT>(a.q, at), f);
       if constexpr (DT == VELOGRAD_DTYPE_F32) Codec<DT>::unpack(load16_any<DT>(a.q, at + 4), f + 4);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= a.q_factor;
     split_parts<S::kQParts>(f, qf[s]);
   }
 }
@@ -596,9 +695,10 @@ __device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, 
 
 // Keys from .. end - 1 (from a multiple of 32) of the tile's sequence and kv head h.  All rows see the keys
 // below `clear`, the last of them those below `most`.  PARTS: of the probabilities.
-template <int D, int FMT, int DT, int NQ, int PARTS>
+// STAGES: tiles of the ring in LDS, or 0 to read codes straight into registers, a tile ahead.
+template <int D, int FMT, int DT, int NQ, int PARTS, int STAGES>
 __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int32_t h, int32_t from, int32_t end,
-                                       int32_t clear, int32_t most, QueryRows<D, FMT, DT, NQ>& rows) {
+                                       int32_t clear, int32_t most, QueryRows<D, FMT, DT, NQ>& rows, uint8_t* ring) {
   using S = Shape<D, FMT, DT>;
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int32_t page_mask = (1 << a.page_shift) - 1;
@@ -642,7 +742,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
 #pragma unroll
               for (int p = S::kQParts - 1; p >= 0; --p) sc = mfma(kf[u][s], rows.frag[q][s][p], sc);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[q][4 * u + i] = sc[i] * a.scale_log2;
+            for (int i = 0; i < 4; ++i) x[q][4 * u + i] = sc[i];
           }
       }
       const uint32_t gone = (uint32_t)(missing >> ((t0 - run) / kHalf)) & 3u;
@@ -675,7 +775,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
       u32x4 pf[NQ][PARTS];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        softmax_step<D>(x[q], rows.state[q]);
+        softmax_step<D>(x[q], a.scale_log2, rows.state[q]);
         split_probs<PARTS>(x[q], pf[q]);
       }
 #pragma unroll
@@ -691,16 +791,41 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
               rows.state[q].acc[2 * d + e] = mfma(vf[e], pf[q][p], rows.state[q].acc[2 * d + e]);
       }
     };
-    // Each step's loads are issued a step before, without a branch around them (past the run's end the last
-    // step's again): the wait for one step's codes then leaves the next one's in flight.
     const int32_t final = run + (run_end - 1 - run) / kTile * kTile;
-    KeyTile<D, FMT> t0, t1;
-    fetch(run, t0);
-    for (int32_t t = run; t <= final; t += 2 * kTile) {
-      fetch(t + kTile < final ? t + kTile : final, t1);
-      use(t, t0);
-      fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
-      if (t + kTile <= final) use(t + kTile, t1);
+    if constexpr (STAGES > 0) {
+      using T = Stage<D, FMT>;
+      uint32_t put = 0, get = 0;  // bytes into the ring
+      auto stage = [&](int32_t t0) {
+        const int32_t t1 = t0 < final ? t0 : final, i = (t1 - run) / kHalf;
+        stage_tile<D, FMT>(a, take_lane(code, i), take_lane(code, i + 1), take_lane(scale, i), take_lane(scale, i + 1),
+                           ring + put);
+        put = put == (STAGES - 1) * T::kBytes ? 0 : put + T::kBytes;
+      };
+#pragma unroll
+      for (int i = 0; i < STAGES - 1; ++i) stage(run + i * kTile);
+      for (int32_t t = run; t <= final; t += kTile) {
+        // Past the run's end the last tile is copied again, so that the count of loads is the same for all.
+        stage(t + (STAGES - 1) * kTile);
+        wait_loads<(STAGES - 1) * T::kLoads>();
+        KeyTile<D, FMT> tile;
+        read_stage<D, FMT>(ring + get, n, g, tile);
+        get = get == (STAGES - 1) * T::kBytes ? 0 : get + T::kBytes;
+        use(t, tile);
+        // The next copy overwrites what was read here.
+        wait_loads<(STAGES - 1) * T::kLoads>();
+      }
+      wait_loads<0>();
+    } else {
+      // Each step's loads are issued a step before, without a branch around them (past the run's end the last
+      // step's again): the wait for one step's codes then leaves the next one's in flight.
+      KeyTile<D, FMT> t0, t1;
+      fetch(run, t0);
+      for (int32_t t = run; t <= final; t += 2 * kTile) {
+        fetch(t + kTile < final ? t + kTile : final, t1);
+        use(t, t0);
+        fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
+        if (t + kTile <= final) use(t + kTile, t1);
+      }
     }
   }
 }
@@ -714,6 +839,9 @@ __device__ __forceinline__ RowTile uniform_rows(const AttnArgs& a, int32_t i) {
   return r;
 }
 
+// Tiles of a wave's ring: the card's waves (step_occupancy) share 160 KiB of LDS.
+constexpr int step_stages(int dim, int fmt) { return dim * (fmt == VELOGRAD_MX_E4M3 ? 64 : 32) <= 4096 ? 3 : 2; }
+
 // Waves of a SIMD that the step kernel's registers are held to.
 constexpr int step_occupancy(int dim, int query_tiles) { return dim == 256 || query_tiles > 1 ? 1 : 2; }
 
@@ -721,8 +849,11 @@ template <int D, int FMT, int DT, int NQ>
 __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
   using S = Shape<D, FMT, DT>;
   constexpr int kTileRows = kRows * NQ;
-  const int32_t worker = (int32_t)blockIdx.x * kWaves + uniform((int)threadIdx.x >> 6);
+  constexpr int kStages = step_stages(D, FMT);
+  __shared__ __attribute__((aligned(16))) uint8_t rings[kWaves][kStages * Stage<D, FMT>::kBytes];
+  const int32_t wave = uniform((int)threadIdx.x >> 6), worker = (int32_t)blockIdx.x * kWaves + wave;
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  uint8_t* ring = rings[wave];
 
   const Share share = find_share(a, kTileRows, worker);
   const int32_t h = worker % a.kv_heads;
@@ -744,7 +875,7 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
     const int32_t end = from + take * kTile < most ? from + take * kTile : most;
     QueryRows<D, FMT, DT, NQ> rows;
     begin_rows(a, r, h, rows);
-    attend<D, FMT, DT, NQ, S::kPParts>(a, r, h, from, end, clear, most, rows);
+    attend<D, FMT, DT, NQ, S::kPParts, kStages>(a, r, h, from, end, clear, most, rows, ring);
 
     const bool whole = take == all;
     const int64_t part = ((int64_t)worker * 2 + (step > 0 ? 0 : 1)) * kTileRows;
@@ -796,7 +927,7 @@ __global__ __launch_bounds__(kWaves * 64, VG_CHUNK_OCC) void mx_attention_chunk_
   const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
   QueryRows<D, FMT, DT, NQ> rows;
   begin_rows(a, r, h, rows);
-  attend<D, FMT, DT, NQ, kParts>(a, r, h, 0, most, clear, most, rows);
+  attend<D, FMT, DT, NQ, kParts, 0>(a, r, h, 0, most, clear, most, rows, nullptr);
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     rows.state[q].l = across_g(rows.state[q].l, true);
@@ -1070,7 +1201,8 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   a.workers = p.workers;
   a.least_steps = p.least_steps;
   a.step_rows = p.step_rows;
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634074);
+  a.scale_log2 = scale == 0.0f ? 1.0f : (float)(__builtin_fabs((double)scale) * 1.4426950408889634074);
+  a.q_factor = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   switch (dtype) {
     case VELOGRAD_DTYPE_F32: launch_fmt<VELOGRAD_DTYPE_F32>(a, p, head_dim, mx_format, st); break;
