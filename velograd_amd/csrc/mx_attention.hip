@@ -307,12 +307,13 @@ __device__ __forceinline__ GlobalByte* scalar(const uint8_t* p) {
   return q;
 }
 
-// To lane l's 16 (or 4) bytes behind `to`; the last argument marks the data as not to be kept (nt).
+// To lane l's 16 (or 4) bytes behind `to`.  Codes come in whole lines, which are not kept (nt, the last argument);
+// scales in parts of lines, which the next steps find in the caches.
 __device__ __forceinline__ void copy16_to_lds(GlobalByte* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((GlobalVoid*)from, (LdsVoid*)to, 16, 0, 2);
 }
 __device__ __forceinline__ void copy4_to_lds(GlobalByte* from, uint8_t* to) {
-  __builtin_amdgcn_global_load_lds((GlobalVoid*)from, (LdsVoid*)to, 4, 0, 2);
+  __builtin_amdgcn_global_load_lds((GlobalVoid*)from, (LdsVoid*)to, 4, 0, 0);
 }
 
 // Lets at most N loads stay in flight, in order, and LDS reads none.
@@ -412,11 +413,21 @@ struct RowState {
   float m, l;
 };
 
-// Scores x become probabilities; updates m, l, acc.  `c` > 0 is the scale times log2(e).
-template <int D>
+template <int N>
+__device__ __forceinline__ float largest(const float* x) {
+  if constexpr (N == 1) return x[0];
+  else return __builtin_fmaxf(largest<N / 2>(x), largest<N / 2>(x + N / 2));
+}
+template <int N>
+__device__ __forceinline__ float sum(const float* x) {
+  if constexpr (N == 1) return x[0];
+  else return sum<N / 2>(x) + sum<N / 2>(x + N / 2);
+}
+
+// N scores x become probabilities; updates m, l, acc.  `c` > 0 is the scale times log2(e).
+template <int D, int N>
 __device__ __forceinline__ void softmax_step(float* x, float c, RowState<D>& r) {
-  float top = __builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])),
-                              __builtin_fmaxf(__builtin_fmaxf(x[4], x[5]), __builtin_fmaxf(x[6], x[7]))) * c;
+  float top = largest<N>(x) * c;
   // The running maximum moves only when a row's new maximum passes it by 8 (p stays below 2^8, which
   // costs fp32 nothing): most steps rescale nothing.
   if (__ballot(top > r.m + 8.0f) != 0) {
@@ -429,8 +440,8 @@ __device__ __forceinline__ void softmax_step(float* x, float c, RowState<D>& r) 
     for (int j = 0; j < D / 16; ++j) r.acc[j] *= f;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -r.m));
-  r.l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+  for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -r.m));
+  r.l += sum<N>(x);
 }
 
 // Bytes of w that are 0xFF (scales: a block marked NaN), or 0x7F with any sign (e4m3's NaN): bit 7 of each.
@@ -450,8 +461,9 @@ __device__ __forceinline__ bool any_nan(const KeyTile<D, FMT>& t) {
 
 // A NaN among the values of a key that only some of the rows see would reach the others as 0 * NaN: its
 // codes are taken out of the tile, and the rows that do see it get NaN by a product of flags.
-template <int D, int FMT, int NQ>
-__device__ __forceinline__ void keep_nan_apart(KeyTile<D, FMT>& t, const float (*x)[8], RowState<D>* rows) {
+// x0: where the tile's 8 scores lie in a row's N.
+template <int D, int FMT, int NQ, int N>
+__device__ __forceinline__ void keep_nan_apart(KeyTile<D, FMT>& t, const float (*x)[N], int x0, RowState<D>* rows) {
   constexpr int kOut = D / 16;
   constexpr int kEach = FMT == VELOGRAD_MX_E4M3 ? kOut : 1;  // e2m1 has no NaN of its own: blocks only
   u32x4 seen[NQ], blocks;
@@ -461,8 +473,8 @@ __device__ __forceinline__ void keep_nan_apart(KeyTile<D, FMT>& t, const float (
     blocks[i] = ((w & 0xffu) == 0xffu ? 0x3f80u : 0u) | ((w & 0xff00u) == 0xff00u ? 0x3f800000u : 0u);
 #pragma unroll
     for (int q = 0; q < NQ; ++q)
-      seen[q][i] = (x[q][2 * i] != -__builtin_inff() ? 0x3f80u : 0u) |
-                   (x[q][2 * i + 1] != -__builtin_inff() ? 0x3f800000u : 0u);
+      seen[q][i] = (x[q][x0 + 2 * i] != -__builtin_inff() ? 0x3f80u : 0u) |
+                   (x[q][x0 + 2 * i + 1] != -__builtin_inff() ? 0x3f800000u : 0u);
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
@@ -695,10 +707,12 @@ __device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, 
 
 // Keys from .. end - 1 (from a multiple of 32) of the tile's sequence and kv head h.  All rows see the keys
 // below `clear`, the last of them those below `most`.  PARTS: of the probabilities.
-// STAGES: tiles of the ring in LDS, or 0 to read codes straight into registers, a tile ahead.
-template <int D, int FMT, int DT, int NQ, int PARTS, int STAGES>
+// TILES of 32 keys make a step.  STAGES: steps of the ring in LDS, or 0 to read codes straight into registers, a
+// step ahead.
+template <int D, int FMT, int DT, int NQ, int PARTS, int TILES, int STAGES>
 __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int32_t h, int32_t from, int32_t end,
                                        int32_t clear, int32_t most, QueryRows<D, FMT, DT, NQ>& rows, uint8_t* ring) {
+  constexpr int kStep = TILES * kTile;
   using S = Shape<D, FMT, DT>;
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int32_t page_mask = (1 << a.page_shift) - 1;
@@ -727,11 +741,12 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
       load_half<D, FMT>(a, c, take_lane(code, i), take_lane(scale, i), 0, t);
       load_half<D, FMT>(a, c, take_lane(code, i + 1), take_lane(scale, i + 1), 1, t);
     };
-    auto use = [&](int32_t t0, KeyTile<D, FMT>& t) {
-      float x[NQ][8];
-      {
+    auto use = [&](int32_t t0, KeyTile<D, FMT>* t) {
+      float x[NQ][8 * TILES];
+#pragma unroll
+      for (int j = 0; j < TILES; ++j) {
         u32x4 kf[2][S::kSteps];
-        decode_keys<D, FMT>(t, kf);
+        decode_keys<D, FMT>(t[j], kf);
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -742,89 +757,103 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
 #pragma unroll
               for (int p = S::kQParts - 1; p >= 0; --p) sc = mfma(kf[u][s], rows.frag[q][s][p], sc);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[q][4 * u + i] = sc[i];
+            for (int i = 0; i < 4; ++i) x[q][8 * j + 4 * u + i] = sc[i];
           }
       }
-      const uint32_t gone = (uint32_t)(missing >> ((t0 - run) / kHalf)) & 3u;
-      const bool masked = t0 + kTile > clear || gone != 0;
+      const uint32_t gone = (uint32_t)(missing >> ((t0 - run) / kHalf)) & ((1u << 2 * TILES) - 1u);
+      const bool masked = t0 + kStep > (clear < end ? clear : end) || gone != 0;
       if (masked) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2 * TILES; ++u) {
           const bool bad = (gone >> u) & 1u;
           const int32_t first = t0 + kHalf * u + 4 * g;
+          KeyTile<D, FMT>& k = t[u / 2];
           // Of the lane's 4 keys: how many there are, and how many the row sees.
-          const int32_t here = bad ? 0 : r.length - first;
+          const int32_t here = bad ? 0 : (r.length < end ? r.length : end) - first;
 #pragma unroll
           for (int q = 0; q < NQ; ++q) {
-            const int32_t see = bad ? 0 : rows.limit[q] - first;
+            const int32_t see = bad ? 0 : (rows.limit[q] < end ? rows.limit[q] : end) - first;
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[q][4 * u + i] = i < see ? x[q][4 * u + i] : -__builtin_inff();
           }
-          // What lies behind the sequence's end may be anything: it is taken as zeros.
+          // What lies behind the sequence's end (or another wave's beginning) is taken as zeros.
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
+            const int at = 4 * (u & 1) + i;
 #pragma unroll
-            for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w)
-              t.vw[4 * u + i][w] = i < here ? t.vw[4 * u + i][w] : 0;
+            for (int w = 0; w < KeyTile<D, FMT>::kWordsV; ++w) k.vw[at][w] = i < here ? k.vw[at][w] : 0;
             const uint32_t m = 0xffu << (8 * i);
-            t.vs[u] = i < here ? t.vs[u] : (t.vs[u] & ~m) | (0x7f7f7f7fu & m);
+            k.vs[u & 1] = i < here ? k.vs[u & 1] : (k.vs[u & 1] & ~m) | (0x7f7f7f7fu & m);
           }
         }
+        if (clear < most) {
+#pragma unroll
+          for (int j = 0; j < TILES; ++j)
+            if (any_nan<D, FMT>(t[j])) keep_nan_apart<D, FMT, NQ, 8 * TILES>(t[j], x, 8 * j, rows.state);
+        }
       }
-      if (masked && clear < most && any_nan<D, FMT>(t)) keep_nan_apart<D, FMT, NQ>(t, x, rows.state);
-      u32x4 pf[NQ][PARTS];
+      u32x4 pf[NQ][TILES][PARTS];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) {
-        softmax_step<D>(x[q], a.scale_log2, rows.state[q]);
-        split_probs<PARTS>(x[q], pf[q]);
+        softmax_step<D, 8 * TILES>(x[q], a.scale_log2, rows.state[q]);
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) split_probs<PARTS>(x[q] + 8 * j, pf[q][j]);
       }
 #pragma unroll
-      for (int d = 0; d < S::kOut / 2; ++d) {
-        u32x4 vf[2];
-        decode_values<D, FMT>(t, d, vf);
+      for (int d = 0; d < S::kOut / 2; ++d)
 #pragma unroll
-        for (int q = 0; q < NQ; ++q)
+        for (int j = 0; j < TILES; ++j) {
+          u32x4 vf[2];
+          decode_values<D, FMT>(t[j], d, vf);
 #pragma unroll
-          for (int p = PARTS - 1; p >= 0; --p)
+          for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              rows.state[q].acc[2 * d + e] = mfma(vf[e], pf[q][p], rows.state[q].acc[2 * d + e]);
-      }
+            for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                rows.state[q].acc[2 * d + e] = mfma(vf[e], pf[q][j][p], rows.state[q].acc[2 * d + e]);
+        }
     };
     const int32_t final = run + (run_end - 1 - run) / kTile * kTile;
     if constexpr (STAGES > 0) {
       using T = Stage<D, FMT>;
+      constexpr uint32_t kBytes = TILES * T::kBytes;
       uint32_t put = 0, get = 0;  // bytes into the ring
       auto stage = [&](int32_t t0) {
-        const int32_t t1 = t0 < final ? t0 : final, i = (t1 - run) / kHalf;
-        stage_tile<D, FMT>(a, take_lane(code, i), take_lane(code, i + 1), take_lane(scale, i), take_lane(scale, i + 1),
-                           ring + put);
-        put = put == (STAGES - 1) * T::kBytes ? 0 : put + T::kBytes;
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) {
+          const int32_t t1 = t0 + j * kTile < final ? t0 + j * kTile : final, i = (t1 - run) / kHalf;
+          stage_tile<D, FMT>(a, take_lane(code, i), take_lane(code, i + 1), take_lane(scale, i),
+                             take_lane(scale, i + 1), ring + put + j * T::kBytes);
+        }
+        put = put == (STAGES - 1) * kBytes ? 0 : put + kBytes;
       };
 #pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) stage(run + i * kTile);
-      for (int32_t t = run; t <= final; t += kTile) {
-        // Past the run's end the last tile is copied again, so that the count of loads is the same for all.
-        stage(t + (STAGES - 1) * kTile);
-        wait_loads<(STAGES - 1) * T::kLoads>();
-        KeyTile<D, FMT> tile;
-        read_stage<D, FMT>(ring + get, n, g, tile);
-        get = get == (STAGES - 1) * T::kBytes ? 0 : get + T::kBytes;
-        use(t, tile);
+      for (int i = 0; i < STAGES - 1; ++i) stage(run + i * kStep);
+      for (int32_t t = run; t <= final; t += kStep) {
+        // Past the run's end its last tile is copied again, so that the count of loads is the same for all.
+        stage(t + (STAGES - 1) * kStep);
+        wait_loads<(STAGES - 1) * TILES * T::kLoads>();
+        KeyTile<D, FMT> tiles[TILES];
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) read_stage<D, FMT>(ring + get + j * T::kBytes, n, g, tiles[j]);
+        get = get == (STAGES - 1) * kBytes ? 0 : get + kBytes;
+        use(t, tiles);
         // The next copy overwrites what was read here.
-        wait_loads<(STAGES - 1) * T::kLoads>();
+        wait_loads<(STAGES - 1) * TILES * T::kLoads>();
       }
       wait_loads<0>();
     } else {
       // Each step's loads are issued a step before, without a branch around them (past the run's end the last
       // step's again): the wait for one step's codes then leaves the next one's in flight.
+      static_assert(TILES == 1, "straight into registers, a step is one tile");
       KeyTile<D, FMT> t0, t1;
       fetch(run, t0);
       for (int32_t t = run; t <= final; t += 2 * kTile) {
         fetch(t + kTile < final ? t + kTile : final, t1);
-        use(t, t0);
+        use(t, &t0);
         fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
-        if (t + kTile <= final) use(t + kTile, t1);
+        if (t + kTile <= final) use(t + kTile, &t1);
       }
     }
   }
@@ -839,8 +868,11 @@ __device__ __forceinline__ RowTile uniform_rows(const AttnArgs& a, int32_t i) {
   return r;
 }
 
-// Tiles of a wave's ring: the card's waves (step_occupancy) share 160 KiB of LDS.
-constexpr int step_stages(int dim, int fmt) { return dim * (fmt == VELOGRAD_MX_E4M3 ? 64 : 32) <= 4096 ? 3 : 2; }
+// Tiles of a step: two where a ring of two steps leaves LDS for the card's waves (step_occupancy) and the
+// registers hold them.
+constexpr int step_tiles(int dim, int fmt, int query_tiles) {
+  return dim * (fmt == VELOGRAD_MX_E4M3 ? 64 : 32) <= 4096 && query_tiles <= 2 ? 2 : 1;
+}
 
 // Waves of a SIMD that the step kernel's registers are held to.
 constexpr int step_occupancy(int dim, int query_tiles) { return dim == 256 || query_tiles > 1 ? 1 : 2; }
@@ -849,8 +881,8 @@ template <int D, int FMT, int DT, int NQ>
 __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
   using S = Shape<D, FMT, DT>;
   constexpr int kTileRows = kRows * NQ;
-  constexpr int kStages = step_stages(D, FMT);
-  __shared__ __attribute__((aligned(16))) uint8_t rings[kWaves][kStages * Stage<D, FMT>::kBytes];
+  constexpr int kStages = 2, kTiles = step_tiles(D, FMT, NQ);
+  __shared__ __attribute__((aligned(16))) uint8_t rings[kWaves][kStages * kTiles * Stage<D, FMT>::kBytes];
   const int32_t wave = uniform((int)threadIdx.x >> 6), worker = (int32_t)blockIdx.x * kWaves + wave;
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   uint8_t* ring = rings[wave];
@@ -875,7 +907,7 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
     const int32_t end = from + take * kTile < most ? from + take * kTile : most;
     QueryRows<D, FMT, DT, NQ> rows;
     begin_rows(a, r, h, rows);
-    attend<D, FMT, DT, NQ, S::kPParts, kStages>(a, r, h, from, end, clear, most, rows, ring);
+    attend<D, FMT, DT, NQ, S::kPParts, kTiles, kStages>(a, r, h, from, end, clear, most, rows, ring);
 
     const bool whole = take == all;
     const int64_t part = ((int64_t)worker * 2 + (step > 0 ? 0 : 1)) * kTileRows;
@@ -927,7 +959,7 @@ __global__ __launch_bounds__(kWaves * 64, VG_CHUNK_OCC) void mx_attention_chunk_
   const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
   QueryRows<D, FMT, DT, NQ> rows;
   begin_rows(a, r, h, rows);
-  attend<D, FMT, DT, NQ, kParts, 0>(a, r, h, 0, most, clear, most, rows, nullptr);
+  attend<D, FMT, DT, NQ, kParts, 1, 0>(a, r, h, 0, most, clear, most, rows, nullptr);
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     rows.state[q].l = across_g(rows.state[q].l, true);
