@@ -1,6 +1,8 @@
 """The MX cache on the GPU: writing (with and without rotation) and reading byte for byte against the
 oracle's quantiser, attention against 64 bits with a bound counted term by term (tests/_mx_cache.py)."""
 
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -199,8 +201,19 @@ def _setup(rng, dt, fmt, dim, heads, kv, page, lengths, fresh, pad, width_extra=
     return parts, table, starts, q
 
 
+@pytest.fixture(params=["short table", "long table"])
+def table_room(request, monkeypatch):
+    """A table with room for few keys lets few rows take one launch, one with room for many is split."""
+    monkeypatch.setattr(sys.modules[__name__], "LONG_TABLE", request.param == "long table")
+
+
+LONG_TABLE = False
+
+
 def _attend(q, parts, table, lengths, starts, fmt, **kw):
     cache = R.from_bytes(parts, fmt, "cuda")
+    if LONG_TABLE:
+        table = np.pad(table, ((0, 0), (0, (1 << 20) // parts[0].shape[2])), constant_values=-9)
     t = torch.from_numpy(table).cuda()
     ln = torch.tensor(lengths, dtype=torch.int32).cuda()
     st = None if starts is None else torch.from_numpy(np.asarray(starts, dtype=np.int32)).cuda()
@@ -246,9 +259,15 @@ ATTENTION = [
     ("bf16", "e2m1", 128, 16, 2, 16, [3000], None, 0),            # split over the keys
     ("fp16", "e2m1", 128, 16, 2, 128, [2500, 1, 900], [2, 1, 7], 2),
     ("fp32", "e2m1", 64, 8, 1, 16, [4100, 5], None, 0),
+    # many sequences, of very unequal lengths
+    ("bf16", "e2m1", 64, 2, 1, 16, [1 + 7 * i % 50 + (1500 if i % 67 == 66 else 0) for i in range(300)], None, 0),
+    ("fp16", "e4m3", 64, 4, 2, 16, [9 * i % 40 + (700 if i % 97 == 96 else 0) for i in range(200)],
+     [i % 3 + (30 if i % 50 == 7 else 0) for i in range(200)], 17),
+    ("fp32", "e2m1", 128, 3, 3, 32, [5 + i % 2 for i in range(130)], [1] * 130, 0),
 ]
 
 
+@pytest.mark.usefixtures("table_room")
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype,fmt,dim,heads,kv,page,lengths,fresh,pad", ATTENTION)
 def test_attention(dtype, fmt, dim, heads, kv, page, lengths, fresh, pad, causal):
@@ -305,6 +324,7 @@ def test_chunks_keep_nan_values_from_rows_that_do_not_see_them():
     assert torch.equal(out[..., :32], clean[0][..., :32])
 
 
+@pytest.mark.usefixtures("table_room")
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_attention_scales(scale):
     _say(f"attention scale {scale}")
@@ -314,6 +334,7 @@ def test_attention_scales(scale):
     _check(got, q, parts, table, [90, 33], starts, 16, "e2m1", scale=scale)
 
 
+@pytest.mark.usefixtures("table_room")
 def test_attention_skips_pages_outside_the_cache():
     _say("attention bad pages")
     rng = np.random.default_rng(6)
@@ -327,6 +348,7 @@ def test_attention_skips_pages_outside_the_cache():
     assert (got[0][1:21] == 0).all() and torch.isneginf(got[1][1:21]).all()
 
 
+@pytest.mark.usefixtures("table_room")
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
 @pytest.mark.parametrize("fresh", [[40], [1]])
 def test_attention_nan_keys_and_values_reach_only_rows_that_see_them(fmt, fresh):
@@ -356,6 +378,7 @@ def test_attention_nan_keys_and_values_reach_only_rows_that_see_them(fmt, fresh)
             assert torch.isnan(out[i]).all() and torch.isnan(lse[i]).all(), i
 
 
+@pytest.mark.usefixtures("table_room")
 def test_attention_nan_and_infinite_queries_stay_in_their_row():
     _say("attention NaN queries")
     rng = np.random.default_rng(8)
@@ -372,6 +395,7 @@ def test_attention_nan_and_infinite_queries_stay_in_their_row():
         assert torch.equal(out[~bad], clean[0][~bad]) and torch.equal(lse[~bad], clean[1][~bad])
 
 
+@pytest.mark.usefixtures("table_room")
 def test_attention_rows_of_no_sequence():
     _say("attention rows of no sequence")
     rng = np.random.default_rng(9)

@@ -31,15 +31,9 @@ using namespace vg;
 constexpr int kTile = 32;   // keys of one step
 constexpr int kWaves = 4;   // waves of a workgroup
 constexpr int kRows = 16;   // query rows of a wave
-#ifndef VG_CHUNK_OCC
-#define VG_CHUNK_OCC 1
-#endif
-#ifndef VG_CHUNK_NQ
-#define VG_CHUNK_NQ 4
-#endif
 // Query tiles of a wave at most, so that its rows and their sums fit the registers.
 constexpr int most_tiles(int dim, int dtype) {
-  const int tiles = dtype == VELOGRAD_DTYPE_BF16 ? VG_CHUNK_NQ : dtype == VELOGRAD_DTYPE_F16 ? 4 : 2;
+  const int tiles = dtype == VELOGRAD_DTYPE_BF16 || dtype == VELOGRAD_DTYPE_F16 ? 4 : 2;
   return dim == 256 ? (dtype == VELOGRAD_DTYPE_BF16 ? 2 : 1) : dim == 128 && dtype == VELOGRAD_DTYPE_F16 ? 2 : tiles;
 }
 // Parts of a probability in chunks: the products count there, and one part of 8 bits (off by at most 2^-8 of
@@ -48,7 +42,12 @@ constexpr int chunk_parts(int dtype) {
   return dtype == VELOGRAD_DTYPE_BF16 ? 1 : dtype == VELOGRAD_DTYPE_F16 ? 2 : 3;
 }
 
-constexpr int kLeastSteps = 4;  // of a wave's share
+// Steps of a wave's share at least: one decode step over 2000 keys takes 12.2 us at 1, 11.0 at 2, 12.7 at 4, 14.6 at
+// 8 (fewer shares are joined faster, but last longer).
+constexpr int kLeastSteps = 2;
+// Steps that the beginning of an item counts for: 24 e4m3 sequences take 35.4 us at 0, 31.5 at 4, 30.7 at 6, 30.0 at
+// 10; 64 ragged ones 79.0, 77.5, 76.9 and 79.2.
+constexpr int kBeginSteps = 6;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -72,6 +71,7 @@ struct AttnArgs {
   int32_t causal;
   int32_t workers;         // waves of the step kernel
   int32_t least_steps;     // its smallest share
+  int32_t begin_steps;     // what the beginning of an item counts for
   int32_t step_rows;       // sequences of more rows are the chunk kernel's
   float scale_log2;        // |scale| * log2(e), or 1
   float q_factor;          // what queries are multiplied by: the scale's sign, or 0
@@ -592,7 +592,11 @@ __device__ __forceinline__ int64_t take_lane(int64_t v, int32_t lane) {
 }
 
 // Steps of an item: a tile of rows of one kv head over everything its sequence holds.
-__device__ inline int32_t tile_steps(int32_t length) { return length <= kTile ? 1 : (length + kTile - 1) / kTile; }
+// Beginning an item (queries, pages, the first codes) takes a wave as long as several steps do, and is counted as
+// such: a wave whose share holds the beginnings of several items gets fewer keys.
+__device__ inline int32_t item_steps(const AttnArgs& a, int32_t length) {
+  return a.begin_steps + (length <= kTile ? 1 : (length + kTile - 1) / kTile);
+}
 
 // Row tiles of a sequence in the step kernel; rows of no sequence are all its own.
 __device__ __forceinline__ int32_t row_tiles(const AttnArgs& a, const RowTile& r, int32_t tile_rows) {
@@ -600,7 +604,7 @@ __device__ __forceinline__ int32_t row_tiles(const AttnArgs& a, const RowTile& r
 }
 
 __device__ __forceinline__ int32_t sequence_steps(const AttnArgs& a, const RowTile& r, int32_t tile_rows) {
-  return row_tiles(a, r, tile_rows) * tile_steps(r.length);
+  return row_tiles(a, r, tile_rows) * item_steps(a, r.length);
 }
 
 // Inclusive sums over the wave's lanes.
@@ -666,8 +670,8 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, int32_t tile_rows
       s.rows.fresh = __builtin_amdgcn_readlane(r.fresh, l);
       s.rows.rows = __builtin_amdgcn_readlane(r.rows, l);
       s.rows.length = __builtin_amdgcn_readlane(r.length, l);
-      s.tile = (int32_t)((uint32_t)in / (uint32_t)tile_steps(s.rows.length));
-      s.step = in - s.tile * tile_steps(s.rows.length);
+      s.tile = (int32_t)((uint32_t)in / (uint32_t)item_steps(a, s.rows.length));
+      s.step = in - s.tile * item_steps(a, s.rows.length);
       return s;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -874,11 +878,16 @@ constexpr int step_tiles(int dim, int fmt, int query_tiles) {
   return dim * (fmt == VELOGRAD_MX_E4M3 ? 64 : 32) <= 4096 && query_tiles <= 2 ? 2 : 1;
 }
 
-// Waves of a SIMD that the step kernel's registers are held to.
-constexpr int step_occupancy(int dim, int query_tiles) { return dim == 256 || query_tiles > 1 ? 1 : 2; }
+// Waves of a SIMD that the step kernel's registers are held to (and its LDS allows).
+constexpr int step_occupancy(int dim, int fmt, int dtype, int query_tiles) {
+  const bool small = fmt == VELOGRAD_MX_E2M1, plain = dtype == VELOGRAD_DTYPE_BF16;
+  if (query_tiles == 4) return 1;
+  if (query_tiles == 2) return dim == 64 || (dim == 128 && plain) ? 2 : 1;
+  return dim < 256 || (small && dtype != VELOGRAD_DTYPE_F32) ? 2 : 1;
+}
 
 template <int D, int FMT, int DT, int NQ>
-__global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
   using S = Shape<D, FMT, DT>;
   constexpr int kTileRows = kRows * NQ;
   constexpr int kStages = 2, kTiles = step_tiles(D, FMT, NQ);
@@ -898,13 +907,14 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
       continue;
     }
     r.row0 = tile * kTileRows;
-    const int32_t all = tile_steps(r.length);
+    const int32_t all = item_steps(a, r.length);
     const int32_t take = all - step < left ? all - step : left;
     const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
     const int32_t most = row_limit(a, r, last / a.group);      // keys that the tile's last row sees,
     const int32_t clear = row_limit(a, r, r.row0 / a.group);   // and that all its rows see
-    const int32_t from = step * kTile;
-    const int32_t end = from + take * kTile < most ? from + take * kTile : most;
+    const int32_t from = step > a.begin_steps ? (step - a.begin_steps) * kTile : 0;
+    const int32_t till = step + take > a.begin_steps ? (step + take - a.begin_steps) * kTile : 0;
+    const int32_t end = till < most ? till : most;
     QueryRows<D, FMT, DT, NQ> rows;
     begin_rows(a, r, h, rows);
     attend<D, FMT, DT, NQ, S::kPParts, kTiles, kStages>(a, r, h, from, end, clear, most, rows, ring);
@@ -931,6 +941,86 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
   }
 }
 
+// Row tile `tile` of a grid that has room for every sequence's last, short tile: tiles of sequence i begin at
+// floor(row bound / tile rows) + i.  False where there is none.
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int32_t tile, int32_t tile_rows, RowTile& r) {
+  if (a.starts == nullptr) {
+    const int32_t per = (a.group + tile_rows - 1) / tile_rows;
+    r = uniform_rows(a, tile / per);
+    r.row0 = tile % per * tile_rows;
+    return true;
+  }
+  const int32_t lane = threadIdx.x & 63;
+  int32_t i = -1;
+  for (int32_t i0 = 0; i0 < sequences(a); i0 += 64) {
+    const bool below = i0 + lane < sequences(a) && row_bound(a, i0 + lane) * a.group / tile_rows + i0 + lane <= tile;
+    i += __popcll(__ballot(below));
+  }
+  i = uniform(i);
+  r = uniform_rows(a, i);
+  r.row0 = (tile - (r.tok0 * a.group / tile_rows + i)) * tile_rows;
+  return r.row0 >= 0 && r.row0 < r.rows;
+}
+
+// ------------------------------------------------------------------------------------------
+// Few rows and short sequences: one launch.
+// ------------------------------------------------------------------------------------------
+// A workgroup takes 16 query rows of one kv head and all their keys, its waves a run of them each, and adds up
+// through LDS: where the card has room for all of them, and the keys are few, that saves the joining launch.
+constexpr int item_waves(int dim, int fmt) { return dim == 256 && fmt == VELOGRAD_MX_E4M3 ? 4 : 8; }
+
+template <int D, int FMT, int DT>
+__global__ __launch_bounds__(item_waves(D, FMT) * 64) void mx_attention_item_kernel(const AttnArgs a) {
+  using S = Shape<D, FMT, DT>;
+  constexpr int kAll = item_waves(D, FMT), kTiles = step_tiles(D, FMT, 1), kStages = 2;
+  constexpr int kRing = kStages * kTiles * Stage<D, FMT>::kBytes, kSums = D / 4 + 2;
+  static_assert(kAll / 2 * kSums * 256 <= kAll * kRing, "the sums reuse the rings");
+  __shared__ __attribute__((aligned(16))) uint8_t rings[kAll * kRing];
+  const int32_t wave = uniform((int)threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4;
+  const int32_t h = (int32_t)(blockIdx.x % (uint32_t)a.kv_heads);
+  RowTile r;
+  if (!find_tile(a, (int32_t)(blockIdx.x / (uint32_t)a.kv_heads), kRows, r)) return;
+  const int32_t last = (r.row0 + kRows < r.rows ? r.row0 + kRows : r.rows) - 1;
+  const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
+  const int32_t steps = (most + kTile - 1) / kTile;
+  const int32_t from = steps * wave / kAll * kTile, till = steps * (wave + 1) / kAll * kTile;
+  QueryRows<D, FMT, DT, 1> rows;
+  begin_rows(a, r, h, rows);
+  attend<D, FMT, DT, 1, S::kPParts, kTiles, kStages>(a, r, h, from, till < most ? till : most, clear, most, rows,
+                                                     rings + wave * kRing);
+  // The upper half of the waves hands its sums to the lower, in the accumulators' own layout, until one is left.
+  RowState<D>& mine = rows.state[0];
+  float* buf = reinterpret_cast<float*>(rings);
+#pragma unroll
+  for (int w = kAll / 2; w >= 1; w >>= 1) {
+    __syncthreads();
+    if (wave >= w && wave < 2 * w) {
+      float* to = buf + (wave - w) * kSums * 64 + lane;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[(4 * j + i) * 64] = mine.acc[j][i];
+      to[D / 4 * 64] = mine.m;
+      to[(D / 4 + 1) * 64] = mine.l;
+    }
+    __syncthreads();
+    if (wave < w) {
+      const float* at = buf + wave * kSums * 64 + lane;
+      const float mo = at[D / 4 * 64], next = __builtin_fmaxf(mine.m, mo);
+      const float f = __builtin_amdgcn_exp2f(mine.m - next), fo = __builtin_amdgcn_exp2f(mo - next);
+      mine.m = next;
+      mine.l = mine.l * f + at[(D / 4 + 1) * 64] * fo;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine.acc[j][i] = mine.acc[j][i] * f + at[(4 * j + i) * 64] * fo;
+    }
+  }
+  if (wave != 0) return;
+  mine.l = across_g(mine.l, true);
+  if (rows.ok[0]) store_row<D, DT>(a, mine, rows.orow[0], g);
+}
+
 // ------------------------------------------------------------------------------------------
 // Many rows a sequence: prefill chunks.
 // ------------------------------------------------------------------------------------------
@@ -938,23 +1028,16 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, NQ)) void mx_attenti
 // Its waves walk the keys together, so the codes that one fetches the others find in the caches; the row
 // tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
 template <int D, int FMT, int DT, int NQ>
-__global__ __launch_bounds__(kWaves * 64, VG_CHUNK_OCC) void mx_attention_chunk_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, 1) void mx_attention_chunk_kernel(const AttnArgs a) {
   constexpr int kTileRows = kRows * NQ, kGroupRows = kWaves * kTileRows;
   constexpr int kParts = chunk_parts(DT);
   const int32_t h = (int32_t)(blockIdx.x % (uint32_t)a.kv_heads);
   const int32_t tile = (int32_t)((gridDim.x - 1 - blockIdx.x) / (uint32_t)a.kv_heads);
-  // Tiles of sequence i begin at floor(row bound / rows of a tile) + i: room for each one's last, short tile.
   const int32_t lane = threadIdx.x & 63, g = lane >> 4;
-  int32_t i = -1;
-  for (int32_t i0 = 0; i0 < sequences(a); i0 += 64) {
-    const bool below = i0 + lane < sequences(a) && row_bound(a, i0 + lane) * a.group / kGroupRows + i0 + lane <= tile;
-    i += __popcll(__ballot(below));
-  }
-  i = uniform(i);
-  RowTile r = uniform_rows(a, i);
-  if (r.seq < 0 || r.rows <= a.step_rows) return;
-  r.row0 = (tile - (r.tok0 * a.group / kGroupRows + i)) * kGroupRows + uniform((int)threadIdx.x >> 6) * kTileRows;
-  if (r.row0 < 0 || r.row0 >= r.rows) return;
+  RowTile r;
+  if (!find_tile(a, tile, kGroupRows, r) || r.seq < 0 || r.rows <= a.step_rows) return;
+  r.row0 += uniform((int)threadIdx.x >> 6) * kTileRows;
+  if (r.row0 >= r.rows) return;
   const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
   const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
   QueryRows<D, FMT, DT, NQ> rows;
@@ -1037,18 +1120,17 @@ __global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a
 struct AttnPlan {
   int32_t query_tiles;  // of a wave of the step kernel: 1, 2 or 4
   int32_t workers;      // its waves
-  int32_t least_steps;
+  int32_t least_steps, begin_steps;
   int32_t step_rows;    // sequences of more rows go to the chunk kernel
   int64_t chunk_tiles;  // its workgroups for each kv head; 0: not launched
-  bool steps;           // whether the step kernel is launched
+  int64_t items;        // workgroups of the item kernel, which then runs alone; or 0
 };
 
 AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                        int32_t dtype, bool ragged, int cus) {
+                        int32_t fmt, int32_t dtype, bool ragged, int64_t table_keys, int cus) {
   AttnPlan p;
   const int64_t group = q_heads / kv_heads, tiles = most_tiles((int)head_dim, dtype);
   const int64_t chunk_rows = kWaves * kRows * tiles;
-  p.steps = true;
   p.chunk_tiles = 0;
   p.step_rows = INT32_MAX;
   // Chunks where their workgroups fill the card; the step kernel splits the keys where they do not.
@@ -1060,15 +1142,23 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
   const int64_t rows = ragged ? q_tokens * group / (batch > 0 ? batch : 1) : group;
   p.query_tiles = p.chunk_tiles > 0 || rows <= kRows || tiles < 2 ? 1 : rows <= 2 * kRows || tiles < 4 ? 2 : 4;
   // As many waves as the card holds at once: every one runs from the start, with an equal share.
-  p.workers = cus * step_occupancy((int)head_dim, p.query_tiles) * kWaves;
+  p.workers = cus * step_occupancy((int)head_dim, fmt, dtype, p.query_tiles) * kWaves;
   if (p.workers > kMostPieces) p.workers = kMostPieces;
   // At least one share for each head.
   if (p.workers < kv_heads) p.workers = (int32_t)((kv_heads + kWaves - 1) / kWaves * kWaves);
   p.least_steps = kLeastSteps;
+  p.begin_steps = kBeginSteps;
+  // One launch, where the card has room for all items at once and a wave's run of the keys is short: the second
+  // launch costs 4 us, a run of 128 keys of 128 dims as much.  With more items the split's shares grow as well.  One
+  // sequence, 8 kv heads: 500 keys 11.0 us split and 8.1 in one launch, 1000 11.6 and 10.7, 2000 11.5 and 14.8;
+  // 16 sequences: 500 keys 14.7 and 8.9, 2000 20.1 and 15.6, 4000 25.5 and 24.1.
+  const int64_t items = (ragged ? q_tokens * group / kRows + batch + 2 : batch * ((group + kRows - 1) / kRows)) * kv_heads;
+  p.items = items <= cus && table_keys * head_dim <= item_waves((int)head_dim, fmt) * 128 * (128 + items) ? items : 0;
   return p;
 }
 
 size_t workspace_bytes(const AttnPlan& p, int64_t q_tokens, int64_t q_heads, int64_t head_dim) {
+  if (p.items > 0) return 0;
   return (size_t)p.workers * 2 * kRows * (size_t)p.query_tiles * (size_t)(head_dim + 2) * sizeof(float) +
          (size_t)q_tokens * (size_t)q_heads * 2 * sizeof(int32_t);
 }
@@ -1077,6 +1167,10 @@ template <int D, int FMT, int DT>
 void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
   constexpr int kMost = most_tiles(D, DT);
   const dim3 block(kWaves * 64), steps((uint32_t)p.workers / kWaves);
+  if (p.items > 0) {
+    hipLaunchKernelGGL((mx_attention_item_kernel<D, FMT, DT>), dim3((uint32_t)p.items), dim3(item_waves(D, FMT) * 64), 0, st, a);
+    return;
+  }
   if (p.chunk_tiles > 0)
     hipLaunchKernelGGL((mx_attention_chunk_kernel<D, FMT, DT, kMost>),
                        dim3((uint32_t)(p.chunk_tiles * a.kv_heads)), block, 0, st, a);
@@ -1144,8 +1238,8 @@ VELOGRAD_API size_t velograd_mx_cache_attention_workspace_bytes(
     return 0;
   const int cus = cu_count(device);
   if (cus <= 0 || q_tokens == 0) return 0;
-  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, dtype,
-                                    ragged != 0, cus);
+  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, mx_format,
+                                    dtype, ragged != 0, table_width * page_size, cus);
   return workspace_bytes(p, q_tokens, q_heads, head_dim);
 }
 
@@ -1185,11 +1279,12 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
     return fail(VELOGRAD_ERR_DEVICE_QUERY, "%s: hipGetDevice failed", what);
   const int cus = cu_count(device);
   if (cus <= 0) return fail(VELOGRAD_ERR_DEVICE_QUERY, "%s: cannot query device %d", what, device);
-  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, dtype, ragged, cus);
+  const AttnPlan p = plan_attention(q_tokens, sequences, q_heads, kv_heads, head_dim, mx_format, dtype, ragged,
+                                    table_width * page_size, cus);
   // The waves count steps in 32 bits: those of the sequences that the step kernel takes.
   const int64_t step_tiles = p.chunk_tiles > 0 ? sequences * ((p.step_rows + kRows - 1) / kRows)
                                                : q_tokens * (q_heads / kv_heads) / kRows + sequences;
-  const int64_t most_steps = table_width * page_size / kTile + 1;
+  const int64_t most_steps = table_width * page_size / kTile + 1 + p.begin_steps;
   if (step_tiles + q_tokens * (q_heads / kv_heads) / kRows + 2 > INT32_MAX / most_steps)
     return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: %lld tokens over %lld pages are too many", what,
                 (long long)q_tokens, (long long)table_width);
@@ -1197,7 +1292,7 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
     return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: %lld row tiles exceed the grid limit", what,
                 (long long)p.chunk_tiles);
   const size_t need = workspace_bytes(p, q_tokens, q_heads, head_dim);
-  if (workspace == nullptr || ws_bytes < need)
+  if (need > 0 && (workspace == nullptr || ws_bytes < need))
     return fail(VELOGRAD_ERR_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
   if (!aligned16(workspace))
     return fail(VELOGRAD_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", what);
@@ -1232,6 +1327,7 @@ VELOGRAD_API int32_t velograd_mx_cache_attention(
   a.causal = causal != 0 ? 1 : 0;
   a.workers = p.workers;
   a.least_steps = p.least_steps;
+  a.begin_steps = p.begin_steps;
   a.step_rows = p.step_rows;
   a.scale_log2 = scale == 0.0f ? 1.0f : (float)(__builtin_fabs((double)scale) * 1.4426950408889634074);
   a.q_factor = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
