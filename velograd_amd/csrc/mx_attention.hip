@@ -22,6 +22,8 @@
 //     keys.  A = V^T: fragment j's row n is dim n D/16 + j, so a lane decodes D/16 consecutive dims of its 8
 //     keys, and pairs keys by one byte permutation for each two elements.
 //   A query row's maximum, sum and rescaling are its lane's own (the four g's share the maximum).
+#include <type_traits>
+
 #include "mx_device.h"
 
 namespace {
@@ -44,6 +46,11 @@ constexpr int chunk_parts(int dtype) {
 
 // Steps of a wave's share at least: one decode step over 2000 keys takes 12.2 us at 1, 11.0 at 2, 12.7 at 4, 14.6 at
 // 8 (fewer shares are joined faster, but last longer).
+// Query tiles of a wave of the chunk kernel, so that its rows, their sums and a step's scores fit 256 registers.
+constexpr int chunk_tiles(int dim, int dtype) {
+  return dim == 64 ? 2 : dim == 128 && dtype != VELOGRAD_DTYPE_F32 ? 2 : 1;
+}
+
 constexpr int kLeastSteps = 2;
 // Steps that the beginning of an item counts for: 24 e4m3 sequences take 35.4 us at 0, 31.5 at 4, 30.7 at 6, 30.0 at
 // 10; 64 ragged ones 79.0, 77.5, 76.9 and 79.2.
@@ -261,28 +268,7 @@ struct KeyTile {
   u32x2 vs;
 };
 
-// Byte offsets of a lane's parts from the first key of a half tile.
-struct LaneView {
-  uint32_t k, ks, v, vs;
-};
-
-// A half's codes and scales; the addresses are the half's, the same for the wave, and the lane's own 32 bits.
-template <int D, int FMT>
-__device__ __forceinline__ void load_half(const AttnArgs& a, const LaneView& c, int64_t code, int64_t scale, int u,
-                                          KeyTile<D, FMT>& t) {
-  using S = typename KeyTile<D, FMT>::S;
-  const uint8_t *kp = a.kc + code, *vp = a.vc + code, *kq = a.ks + scale, *vq = a.vs + scale;
-#pragma unroll
-  for (int i = 0; i < S::kChunks; ++i) {
-    load_words<S::kChunkBytes>(kp + (c.k + 4 * i * S::kChunkBytes), t.kw[u] + i * (S::kChunkBytes / 4));
-    t.ks[u][i] = kq[c.ks + (uint32_t)((i * (S::kChunkElems / 8)) << a.page_shift)];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) load_words<S::kVBytes>(vp + (c.v + i * S::kRowBytes), t.vw[4 * u + i]);
-  t.vs[u] = *reinterpret_cast<const uint32_t*>(vq + c.vs);
-}
-
-// The same tile by way of LDS: copied there without passing registers, 16 bytes a lane from whole lines (past
+// A tile comes by way of LDS: copied there without passing registers, 16 bytes a lane from whole lines (past
 // the caches that nothing else reads it from), kStages - 1 tiles ahead, into a ring of the wave's own.
 template <int D, int FMT>
 struct Stage {
@@ -424,7 +410,25 @@ __device__ __forceinline__ float sum(const float* x) {
   else return sum<N / 2>(x) + sum<N / 2>(x + N / 2);
 }
 
-// N scores x become probabilities; updates m, l, acc.  `c` > 0 is the scale times log2(e).
+// A row's running maximum moves to `next`.
+template <int D>
+__device__ __forceinline__ void set_max(float next, RowState<D>& r) {
+  const float f = __builtin_amdgcn_exp2f(r.m - next);
+  r.m = next;
+  r.l *= f;
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) r.acc[j] *= f;
+}
+
+// Probabilities of N scores; returns their sum.  `c` > 0 is the scale times log2(e).
+template <int N>
+__device__ __forceinline__ float probabilities(const float* x, float* p, float c, float m) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -m));
+  return sum<N>(p);
+}
+
+// N scores x become probabilities; updates m, l, acc.
 template <int D, int N>
 __device__ __forceinline__ void softmax_step(float* x, float c, RowState<D>& r) {
   float top = largest<N>(x) * c;
@@ -432,16 +436,9 @@ __device__ __forceinline__ void softmax_step(float* x, float c, RowState<D>& r) 
   // costs fp32 nothing): most steps rescale nothing.
   if (__ballot(top > r.m + 8.0f) != 0) {
     top = across_g(top, false);
-    const float next = top > r.m + 8.0f ? top : r.m;  // for each row by itself
-    const float f = __builtin_amdgcn_exp2f(r.m - next);
-    r.m = next;
-    r.l *= f;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) r.acc[j] *= f;
+    set_max<D>(top > r.m + 8.0f ? top : r.m, r);  // for each row by itself
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -r.m));
-  r.l += sum<N>(x);
+  r.l += probabilities<N>(x, x, c, r.m);
 }
 
 // Bytes of w that are 0xFF (scales: a block marked NaN), or 0x7F with any sign (e4m3's NaN): bit 7 of each.
@@ -552,13 +549,13 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, const RowState<D>& 
 }
 
 // A query row's fragments, in the order of decode_keys; zeros for a row that is none.
-template <int D, int FMT, int DT>
+template <int D, int FMT, int DT, int CHUNK>
 __device__ __forceinline__ void load_query(const AttnArgs& a, int64_t e, int32_t g, bool ok,
                                            u32x4 (*qf)[Shape<D, FMT, DT>::kQParts]) {
   using S = Shape<D, FMT, DT>;
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
-    const int64_t at = e + (4 * (8 * s / S::kChunkElems) + g) * S::kChunkElems + 8 * s % S::kChunkElems;
+    const int64_t at = e + (4 * (8 * s / CHUNK) + g) * CHUNK + 8 * s % CHUNK;
     if constexpr (S::kQParts == 1) {
       qf[s][0] = u32x4{0u, 0u, 0u, 0u};
       if (ok) qf[s][0] = load16_any<DT>(a.q, at);
@@ -688,7 +685,7 @@ struct QueryRows {
   RowState<D> state[NQ];
 };
 
-template <int D, int FMT, int DT, int NQ>
+template <int CHUNK, int D, int FMT, int DT, int NQ>
 __device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, int32_t h,
                                            QueryRows<D, FMT, DT, NQ>& w) {
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -701,7 +698,7 @@ __device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, 
     w.limit[q] = w.ok[q] ? row_limit(a, r, fresh) : 0;
     const int64_t tok = r.tok0 + fresh;
     w.orow[q] = tok * a.q_heads + head;
-    load_query<D, FMT, DT>(a, tok * a.q_t + head * a.q_h, g, w.ok[q], w.frag[q]);
+    load_query<D, FMT, DT, CHUNK>(a, tok * a.q_t + head * a.q_h, g, w.ok[q], w.frag[q]);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) w.state[q].acc[j] = f32x4{0, 0, 0, 0};
     w.state[q].m = -3.0e38f;
@@ -711,8 +708,7 @@ __device__ __forceinline__ void begin_rows(const AttnArgs& a, const RowTile& r, 
 
 // Keys from .. end - 1 (from a multiple of 32) of the tile's sequence and kv head h.  All rows see the keys
 // below `clear`, the last of them those below `most`.  PARTS: of the probabilities.
-// TILES of 32 keys make a step.  STAGES: steps of the ring in LDS, or 0 to read codes straight into registers, a
-// step ahead.
+// TILES of 32 keys make a step, STAGES steps the ring in LDS.
 template <int D, int FMT, int DT, int NQ, int PARTS, int TILES, int STAGES>
 __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int32_t h, int32_t from, int32_t end,
                                        int32_t clear, int32_t most, QueryRows<D, FMT, DT, NQ>& rows, uint8_t* ring) {
@@ -721,11 +717,6 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
   const int32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int32_t page_mask = (1 << a.page_shift) - 1;
   const int32_t* table = a.table + (int64_t)(r.seq < 0 ? 0 : r.seq) * a.table_stride;
-  LaneView c;
-  c.k = n * S::kRowBytes + g * S::kChunkBytes;
-  c.v = 4 * g * S::kRowBytes + n * S::kVBytes;
-  c.ks = (((g * S::kChunkElems) / 32) << a.page_shift) + n;
-  c.vs = (((n * (D / 16)) / 32) << a.page_shift) + 4 * g;
 
   for (int32_t run = from; run < end; run += kRunKeys) {
     const int32_t run_end = run + kRunKeys < end ? run + kRunKeys : end;
@@ -740,11 +731,6 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
     const int64_t code = ((paged << a.page_shift) + place) * S::kRowBytes;
     const int64_t scale = ((paged * (D / 32)) << a.page_shift) + place;
 
-    auto fetch = [&](int32_t t0, KeyTile<D, FMT>& t) {
-      const int32_t i = (t0 - run) / kHalf;
-      load_half<D, FMT>(a, c, take_lane(code, i), take_lane(scale, i), 0, t);
-      load_half<D, FMT>(a, c, take_lane(code, i + 1), take_lane(scale, i + 1), 1, t);
-    };
     auto use = [&](int32_t t0, KeyTile<D, FMT>* t) {
       float x[NQ][8 * TILES];
 #pragma unroll
@@ -819,47 +805,33 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const RowTile& r, int3
         }
     };
     const int32_t final = run + (run_end - 1 - run) / kTile * kTile;
-    if constexpr (STAGES > 0) {
-      using T = Stage<D, FMT>;
-      constexpr uint32_t kBytes = TILES * T::kBytes;
-      uint32_t put = 0, get = 0;  // bytes into the ring
-      auto stage = [&](int32_t t0) {
+    using T = Stage<D, FMT>;
+    constexpr uint32_t kBytes = TILES * T::kBytes;
+    uint32_t put = 0, get = 0;  // bytes into the ring
+    auto stage = [&](int32_t t0) {
 #pragma unroll
-        for (int j = 0; j < TILES; ++j) {
-          const int32_t t1 = t0 + j * kTile < final ? t0 + j * kTile : final, i = (t1 - run) / kHalf;
-          stage_tile<D, FMT>(a, take_lane(code, i), take_lane(code, i + 1), take_lane(scale, i),
-                             take_lane(scale, i + 1), ring + put + j * T::kBytes);
-        }
-        put = put == (STAGES - 1) * kBytes ? 0 : put + kBytes;
-      };
-#pragma unroll
-      for (int i = 0; i < STAGES - 1; ++i) stage(run + i * kStep);
-      for (int32_t t = run; t <= final; t += kStep) {
-        // Past the run's end its last tile is copied again, so that the count of loads is the same for all.
-        stage(t + (STAGES - 1) * kStep);
-        wait_loads<(STAGES - 1) * TILES * T::kLoads>();
-        KeyTile<D, FMT> tiles[TILES];
-#pragma unroll
-        for (int j = 0; j < TILES; ++j) read_stage<D, FMT>(ring + get + j * T::kBytes, n, g, tiles[j]);
-        get = get == (STAGES - 1) * kBytes ? 0 : get + kBytes;
-        use(t, tiles);
-        // The next copy overwrites what was read here.
-        wait_loads<(STAGES - 1) * TILES * T::kLoads>();
+      for (int j = 0; j < TILES; ++j) {
+        const int32_t t1 = t0 + j * kTile < final ? t0 + j * kTile : final, i = (t1 - run) / kHalf;
+        stage_tile<D, FMT>(a, take_lane(code, i), take_lane(code, i + 1), take_lane(scale, i),
+                           take_lane(scale, i + 1), ring + put + j * T::kBytes);
       }
-      wait_loads<0>();
-    } else {
-      // Each step's loads are issued a step before, without a branch around them (past the run's end the last
-      // step's again): the wait for one step's codes then leaves the next one's in flight.
-      static_assert(TILES == 1, "straight into registers, a step is one tile");
-      KeyTile<D, FMT> t0, t1;
-      fetch(run, t0);
-      for (int32_t t = run; t <= final; t += 2 * kTile) {
-        fetch(t + kTile < final ? t + kTile : final, t1);
-        use(t, &t0);
-        fetch(t + 2 * kTile < final ? t + 2 * kTile : final, t0);
-        if (t + kTile <= final) use(t + kTile, &t1);
-      }
+      put = put == (STAGES - 1) * kBytes ? 0 : put + kBytes;
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) stage(run + i * kStep);
+    for (int32_t t = run; t <= final; t += kStep) {
+      // Past the run's end its last tile is copied again, so that the count of loads is the same for all.
+      stage(t + (STAGES - 1) * kStep);
+      wait_loads<(STAGES - 1) * TILES * T::kLoads>();
+      KeyTile<D, FMT> tiles[TILES];
+#pragma unroll
+      for (int j = 0; j < TILES; ++j) read_stage<D, FMT>(ring + get + j * T::kBytes, n, g, tiles[j]);
+      get = get == (STAGES - 1) * kBytes ? 0 : get + kBytes;
+      use(t, tiles);
+      // The next copy overwrites what was read here.
+      wait_loads<(STAGES - 1) * TILES * T::kLoads>();
     }
+    wait_loads<0>();
   }
 }
 
@@ -916,7 +888,7 @@ __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT, NQ)) void m
     const int32_t till = step + take > a.begin_steps ? (step + take - a.begin_steps) * kTile : 0;
     const int32_t end = till < most ? till : most;
     QueryRows<D, FMT, DT, NQ> rows;
-    begin_rows(a, r, h, rows);
+    begin_rows<S::kChunkElems>(a, r, h, rows);
     attend<D, FMT, DT, NQ, S::kPParts, kTiles, kStages>(a, r, h, from, end, clear, most, rows, ring);
 
     const bool whole = take == all;
@@ -985,7 +957,7 @@ __global__ __launch_bounds__(item_waves(D, FMT) * 64) void mx_attention_item_ker
   const int32_t steps = (most + kTile - 1) / kTile;
   const int32_t from = steps * wave / kAll * kTile, till = steps * (wave + 1) / kAll * kTile;
   QueryRows<D, FMT, DT, 1> rows;
-  begin_rows(a, r, h, rows);
+  begin_rows<S::kChunkElems>(a, r, h, rows);
   attend<D, FMT, DT, 1, S::kPParts, kTiles, kStages>(a, r, h, from, till < most ? till : most, clear, most, rows,
                                                      rings + wave * kRing);
   // The upper half of the waves hands its sums to the lower, in the accumulators' own layout, until one is left.
@@ -1024,25 +996,328 @@ __global__ __launch_bounds__(item_waves(D, FMT) * 64) void mx_attention_item_ker
 // ------------------------------------------------------------------------------------------
 // Many rows a sequence: prefill chunks.
 // ------------------------------------------------------------------------------------------
-// A workgroup takes 64 NQ consecutive rows of one kv head over all the keys they see, a wave 16 NQ of them.
-// Its waves walk the keys together, so the codes that one fetches the others find in the caches; the row
-// tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
+// A workgroup takes 128 NQ consecutive rows of one kv head over all the keys they see, a wave 16 NQ of them.  All
+// waves decode a step's keys together, a thread 16 elements of a key and 4 dims of 4 values, into LDS in the order
+// of the products' operands; each step's codes are loaded a step before they are decoded, so one barrier a step is
+// left.  The row tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
+constexpr int kChunkWaves = 8;
+
+// The codes of a thread's keys and values of one step.
+template <int D, int FMT>
+struct ChunkCodes {
+  static constexpr int kWordsK = FMT == VELOGRAD_MX_E2M1 ? 2 : 4;
+  uint32_t kw[kWordsK], vw[4], ks, vs;
+  bool bad;  // the keys' page is not in the cache
+};
+
+template <int D, int FMT>
+struct ChunkPlace {
+  static constexpr int kKeys = 16 * kChunkWaves * 64 / D;  // of a step
+  static constexpr int kLanes = D / 4;                     // threads of 4 keys
+  int32_t quad, c;      // first of the 4 keys in the step; dims 4 c .. of the values
+  int32_t key, chunk;   // its key and the 16 elements of it
+  int32_t h;
+};
+
+template <int D, int FMT>
+__device__ __forceinline__ void load_codes(const AttnArgs& a, const ChunkPlace<D, FMT>& w, int32_t page, int32_t t0,
+                                           ChunkCodes<D, FMT>& t) {
+  constexpr int kRowBytes = FMT == VELOGRAD_MX_E2M1 ? D / 2 : D;
+  t.bad = (uint32_t)page >= (uint32_t)a.pages;
+  const int64_t base = (int64_t)(t.bad ? 0 : page) * a.kv_heads + w.h;
+  const int32_t place = (t0 + w.quad) & ((1 << a.page_shift) - 1);
+  const int64_t code = ((base << a.page_shift) + place) * kRowBytes;
+  const int64_t scale = ((base * (D / 32)) << a.page_shift) + place;
+  const uint8_t* kc = a.kc + code + (w.key - w.quad) * kRowBytes + w.chunk * (16 * kRowBytes / D);
+  const uint8_t* vc = a.vc + code + w.c * (4 * kRowBytes / D);
+  if constexpr (FMT == VELOGRAD_MX_E2M1) {
+    const u32x2 k = *reinterpret_cast<const u32x2*>(kc);
+    t.kw[0] = k[0];
+    t.kw[1] = k[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.vw[i] = *reinterpret_cast<const uint16_t*>(vc + i * kRowBytes);
+  } else {
+    const u32x4 k = *reinterpret_cast<const u32x4*>(kc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.kw[i] = k[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.vw[i] = *reinterpret_cast<const uint32_t*>(vc + i * kRowBytes);
+  }
+  t.ks = a.ks[scale + ((int64_t)(w.chunk / 2) << a.page_shift) + (w.key - w.quad)];
+  t.vs = *reinterpret_cast<const uint32_t*>(a.vs + scale + ((int64_t)(w.c / 8) << a.page_shift));
+}
+
+// Of a step's keys in LDS: the operands of S^T and of O^T, and for each 16 keys whether their page is missing.
+template <int D>
+struct ChunkStage {
+  static constexpr int kKeys = 16 * kChunkWaves * 64 / D, kTiles = kKeys / kTile;
+  u32x4 k[kTiles][2][D / 32][64];
+  u32x4 v[kTiles][D / 16][64];
+  uint8_t gone[16];
+};
+
+// Keys from `end` on, and those of missing pages, are decoded to zeros.
+template <int D, int FMT>
+__device__ __forceinline__ void put_codes(const ChunkPlace<D, FMT>& w, ChunkCodes<D, FMT>& t, int32_t t0, int32_t end,
+                                          ChunkStage<D>& st) {
+  constexpr int kOut = D / 16, kPerWord = FMT == VELOGRAD_MX_E2M1 ? 4 : 2;
+  if (t0 + ChunkStage<D>::kKeys > end || __ballot(t.bad) != 0) {
+    const int32_t here = t.bad ? 0 : end - t0;
+    if (w.key >= here) {
+#pragma unroll
+      for (int i = 0; i < ChunkCodes<D, FMT>::kWordsK; ++i) t.kw[i] = 0;
+      t.ks = 127;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = 0xffu << (8 * i);
+      if (w.quad + i >= here) {
+        t.vw[i] = 0;
+        t.vs = (t.vs & ~m) | (0x7f7f7f7fu & m);
+      }
+    }
+  }
+  if (w.c == 0 && w.quad % kHalf == 0) st.gone[w.quad / kHalf] = t.bad ? 1 : 0;
+  const float ks = scale_arg(t.ks);
+  u32x4 e[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i / 4][i % 4] = decode_pair<FMT>(t.kw[i / kPerWord], ks, i % kPerWord);
+  // Lane (n, g) of step s reads column n ^ (4 s + (g & 2)): threads of one key would write to the same banks.
+  u32x4* k = st.k[w.key / kTile][w.key / kHalf % 2][w.chunk / 2];
+  const int32_t g = w.chunk % 2 * 2, n = (w.key % kHalf) ^ (w.chunk * 2 & 15);
+  k[16 * g + n] = e[0];
+  k[16 * g + 16 + n] = e[1];
+  u32x2 x[4];  // 4 dims of 4 keys: pairs of keys
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float s0 = __builtin_bit_cast(float, i == 0 ? t.vs << 23 : t.vs << 7);
+    const float s1 = __builtin_bit_cast(float, i == 0 ? t.vs << 15 : t.vs >> 1);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t u0 = decode_pair<FMT>(t.vw[2 * i], s0, d), u1 = decode_pair<FMT>(t.vw[2 * i + 1], s1, d);
+      x[2 * d][i] = __builtin_amdgcn_perm(u1, u0, 0x05040100u);
+      x[2 * d + 1][i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+    }
+  }
+  const int32_t lane = 16 * (w.quad / 4 % 4) + 4 * w.c / kOut, half = w.quad / kHalf % 2;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    reinterpret_cast<u32x2*>(&st.v[w.quad / kTile][4 * w.c % kOut + d][lane])[half] = x[d];
+}
+
+// A barrier for what lies in LDS: loads into registers stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int D, int FMT, int DT, int NQ>
-__global__ __launch_bounds__(kWaves * 64, 1) void mx_attention_chunk_kernel(const AttnArgs a) {
-  constexpr int kTileRows = kRows * NQ, kGroupRows = kWaves * kTileRows;
+__global__ __launch_bounds__(kChunkWaves * 64, 2) void mx_attention_chunk_kernel(const AttnArgs a) {
+  using S = Shape<D, FMT, DT>;
+  using T = ChunkStage<D>;
+  constexpr int kTileRows = kRows * NQ, kGroupRows = kChunkWaves * kTileRows, kOut = D / 16;
+  constexpr int kGroup = T::kTiles < 2 ? T::kTiles : 2;  // tiles whose scores are held at a time
   constexpr int kParts = chunk_parts(DT);
-  const int32_t h = (int32_t)(blockIdx.x % (uint32_t)a.kv_heads);
-  const int32_t tile = (int32_t)((gridDim.x - 1 - blockIdx.x) / (uint32_t)a.kv_heads);
-  const int32_t lane = threadIdx.x & 63, g = lane >> 4;
+  __shared__ T stages[2];
+  const int32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, wave = uniform(tid >> 6);
+  ChunkPlace<D, FMT> w;
+  w.h = (int32_t)(blockIdx.x % (uint32_t)a.kv_heads);
+  w.quad = tid / w.kLanes * 4;
+  w.c = tid % w.kLanes;
+  w.key = w.quad + w.c / kOut;
+  w.chunk = w.c % kOut;
+  const int32_t item = (int32_t)((gridDim.x - 1 - blockIdx.x) / (uint32_t)a.kv_heads);
   RowTile r;
-  if (!find_tile(a, tile, kGroupRows, r) || r.seq < 0 || r.rows <= a.step_rows) return;
-  r.row0 += uniform((int)threadIdx.x >> 6) * kTileRows;
-  if (r.row0 >= r.rows) return;
-  const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
-  const int32_t most = row_limit(a, r, last / a.group), clear = row_limit(a, r, r.row0 / a.group);
+  if (!find_tile(a, item, kGroupRows, r) || r.seq < 0 || r.rows <= a.step_rows) return;
+  const int32_t group_last = (r.row0 + kGroupRows < r.rows ? r.row0 + kGroupRows : r.rows) - 1;
+  const int32_t end = row_limit(a, r, group_last / a.group);  // keys that any row of the group sees
+  r.row0 += wave * kTileRows;
+  int32_t most = 0, clear = 0;  // of the wave's rows: the last sees, all see
+  if (r.row0 < r.rows) {
+    const int32_t last = (r.row0 + kTileRows < r.rows ? r.row0 + kTileRows : r.rows) - 1;
+    most = row_limit(a, r, last / a.group);
+    clear = row_limit(a, r, r.row0 / a.group);
+  }
   QueryRows<D, FMT, DT, NQ> rows;
-  begin_rows(a, r, h, rows);
-  attend<D, FMT, DT, NQ, kParts, 1, 0>(a, r, h, 0, most, clear, most, rows, nullptr);
+  begin_rows<8>(a, r, w.h, rows);
+
+  const int32_t* table = a.table + (int64_t)r.seq * a.table_stride;
+  auto find_page = [&](int32_t t0) {
+    const int32_t at = (t0 + w.quad) >> a.page_shift;
+    return table[at < a.width ? at : a.width - 1];
+  };
+  auto use = [&](const T& st, int32_t t0, int32_t j0, uint32_t gone, auto masked_step) {
+    constexpr bool kMasked = decltype(masked_step)::value;
+    // Operands are read from LDS in batches of 4, each while the products of the one before run.
+    constexpr int kBatchesK = kGroup * S::kSteps / 2, kBatchesV = kGroup * kOut / 4;
+    u32x4 kf[2][2][2], vf[2][4];
+    auto read_keys = [&](int b) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int s = b % (S::kSteps / 2) * 2 + i;
+          kf[b & 1][i][u] = st.k[j0 + b / (S::kSteps / 2)][u][s][16 * g + (n ^ ((4 * s + (g & 2)) & 15))];
+        }
+    };
+    auto read_values = [&](int b) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vf[b & 1][i] = st.v[j0 + b / (kOut / 4)][b % (kOut / 4) * 4 + i][lane];
+    };
+    float x[NQ][8 * kGroup];
+    f32x4 sc[NQ][2];
+    read_keys(0);
+#pragma unroll
+    for (int b = 0; b < kBatchesK; ++b) {
+      const int s0 = b % (S::kSteps / 2) * 2, j = b / (S::kSteps / 2);
+      if (b + 1 < kBatchesK) read_keys(b + 1);
+      else read_values(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int p = S::kQParts - 1; p >= 0; --p)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+              sc[q][u] = mfma(kf[b & 1][i][u], rows.frag[q][s0 + i][p],
+                              s0 + i == 0 && p == S::kQParts - 1 ? f32x4{0, 0, 0, 0} : sc[q][u]);
+      if (s0 + 2 == S::kSteps)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[q][8 * j + i] = sc[q][i / 4][i % 4];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kMasked) {
+#pragma unroll
+      for (int u = 0; u < 2 * kGroup; ++u)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+          const int32_t see = (gone >> 8 * u & 1u) != 0 ? 0 : rows.limit[q] - (t0 + kHalf * u + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[q][4 * u + i] = i < see ? x[q][4 * u + i] : -__builtin_inff();
+        }
+    }
+    // Probabilities by the running maximum as it is: it has to move only where their sum passes 2^8, which a maximum
+    // behind by 8 brings about by itself, so that no maximum is taken in most steps.
+    float p[NQ][8 * kGroup], l[NQ];
+    bool moves = false;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      l[q] = probabilities<8 * kGroup>(x[q], p[q], a.scale_log2, rows.state[q].m);
+      moves |= l[q] > 256.0f;
+    }
+    if (__ballot(moves) != 0) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const float top = across_g(largest<8 * kGroup>(x[q]) * a.scale_log2, false);
+        const bool own = across_g(l[q], false) > 256.0f;  // each row by itself: its bits do not depend on others'
+        set_max<D>(own ? __builtin_fmaxf(top, rows.state[q].m) : rows.state[q].m, rows.state[q]);
+        l[q] = probabilities<8 * kGroup>(x[q], p[q], a.scale_log2, rows.state[q].m);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) rows.state[q].l += l[q];
+    u32x4 pf[NQ][kParts];
+#pragma unroll
+    for (int b = 0; b < kBatchesV; ++b) {
+      const int j = b / (kOut / 4);
+      if (b + 1 < kBatchesV) read_values(b + 1);
+      if (b % (kOut / 4) == 0)
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) split_probs<kParts>(p[q] + 8 * j, pf[q]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kMasked) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // A NaN among the values that only some of the rows see would reach the others as 0 * NaN: it is taken
+          // out, and the rows that do see it get NaN by a product of flags.
+          const int d = b % (kOut / 4) * 4 + e;
+          u32x4& v = vf[b & 1][e];
+          u32x4 flags;
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool low = (v[i] & 0x7fffu) > 0x7f80u, high = (v[i] & 0x7fffffffu) > 0x7f80ffffu;
+            flags[i] = (low ? 0x3f80u : 0u) | (high ? 0x3f800000u : 0u);
+            v[i] &= (low ? 0u : 0xffffu) | (high ? 0u : 0xffff0000u);
+            any |= flags[i];
+          }
+          if (__ballot(any != 0) == 0) continue;
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            u32x4 seen;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int u = 2 * j + i / 2;
+              const int32_t see =
+                  (gone >> 8 * u & 1u) != 0 ? 0 : rows.limit[q] - (t0 + kHalf * u + 4 * g + 2 * (i & 1));
+              seen[i] = (see > 0 ? 0x3f80u : 0u) | (see > 1 ? 0x3f800000u : 0u);
+            }
+            const f32x4 hit = mfma(flags, seen, f32x4{0, 0, 0, 0});
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              rows.state[q].acc[d][i] = hit[i] > 0.0f ? __builtin_nanf("") : rows.state[q].acc[d][i];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = kParts - 1; i >= 0; --i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            f32x4& acc = rows.state[q].acc[b % (kOut / 4) * 4 + e];
+            acc = mfma(vf[b & 1][e], pf[q][i], acc);
+          }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  ChunkCodes<D, FMT> codes;
+  if (end > 0) {
+    load_codes<D, FMT>(a, w, find_page(0), 0, codes);
+    put_codes<D, FMT>(w, codes, 0, end, stages[0]);
+    load_codes<D, FMT>(a, w, find_page(T::kKeys), T::kKeys, codes);
+  }
+  int32_t page = end > 0 ? find_page(2 * T::kKeys) : 0;
+  int32_t t = 0, at = 0;
+  // A step begins: its keys lie in LDS, those of the one before may be overwritten.  Whether pages are missing
+  // (for each 16 keys a byte of `gone`).
+  constexpr int kWords = (2 * T::kTiles + 3) / 4;
+  constexpr uint32_t kEvery = T::kTiles == 1 ? 0xffffu : 0xffffffffu;
+  uint32_t gone[kWords];
+  auto begin_step = [&]() {
+    lds_barrier();
+    // Past the end the loads go on over the table's last page; nothing uses them.
+    put_codes<D, FMT>(w, codes, t + T::kKeys, end, stages[at ^ 1]);
+    load_codes<D, FMT>(a, w, page, t + 2 * T::kKeys, codes);
+    page = find_page(t + 3 * T::kKeys);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      gone[i] = (uint32_t)uniform(*reinterpret_cast<const int32_t*>(stages[at].gone + 4 * i)) & kEvery;
+    return kWords == 2 ? (gone[0] | gone[1]) != 0 : gone[0] != 0;
+  };
+  // All rows see all keys of the first steps.  The rest, and all from a missing page on, is masked.  Every wave
+  // begins one step more than there are, whichever loop ends its walk.
+  bool any_gone = end > 0 && begin_step();
+  while (t + T::kKeys <= clear && !any_gone) {
+#pragma unroll
+    for (int j = 0; j < T::kTiles; j += kGroup) use(stages[at], t + j * kTile, j, 0, std::false_type{});
+    t += T::kKeys;
+    at ^= 1;
+    any_gone = begin_step();
+  }
+  while (t < end) {
+#pragma unroll
+    for (int j = 0; j < T::kTiles; j += kGroup)
+      if (t + j * kTile < most) use(stages[at], t + j * kTile, j, gone[j / 2], std::true_type{});
+    t += T::kKeys;
+    at ^= 1;
+    begin_step();
+  }
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     rows.state[q].l = across_g(rows.state[q].l, true);
@@ -1054,7 +1329,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void mx_attention_chunk_kernel(cons
 
 // Joins the pieces of the (token, head) rows that have several: a row's first is the last of its wave's share,
 // the others are the first of the shares that follow in the head.  D/4 lanes hold the row, the workgroup's
-// other lanes take other pieces, and LDS adds them up.
+// other lanes take other pieces, and LDS adds them up.  A workgroup's rows lie a grid apart, so that a sequence's rows,
+// split or not split together, go to many workgroups.
 constexpr int kMostPieces = 2048;
 
 template <int D, int DT>
@@ -1066,13 +1342,14 @@ __global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a
   __shared__ int32_t found[256];
   __shared__ int32_t count;
   const int32_t tid = threadIdx.x, d = tid % kLanes, set = tid / kLanes;
-  const int64_t all = (int64_t)a.q_tokens * a.q_heads, row0 = (int64_t)blockIdx.x * rows;
+  const int64_t all = (int64_t)a.q_tokens * a.q_heads;
   if (tid == 0) count = 0;
   __syncthreads();
-  if (tid < rows && row0 + tid < all && (a.joins[(row0 + tid) * 2 + 1] >> 8) > 1) found[atomicAdd(&count, 1)] = tid;
+  const int64_t mine = blockIdx.x + (int64_t)tid * gridDim.x;
+  if (tid < rows && mine < all && (a.joins[mine * 2 + 1] >> 8) > 1) found[atomicAdd(&count, 1)] = tid;
   __syncthreads();
   for (int32_t k = 0; k < count; ++k) {
-    const int64_t orow = row0 + found[k];
+    const int64_t orow = blockIdx.x + (int64_t)found[k] * gridDim.x;
     const int32_t first = a.joins[orow * 2], packed = a.joins[orow * 2 + 1];
     const int32_t active = packed >> 8;
     auto place = [&](int32_t s) {
@@ -1130,7 +1407,7 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
                         int32_t fmt, int32_t dtype, bool ragged, int64_t table_keys, int cus) {
   AttnPlan p;
   const int64_t group = q_heads / kv_heads, tiles = most_tiles((int)head_dim, dtype);
-  const int64_t chunk_rows = kWaves * kRows * tiles;
+  const int64_t chunk_rows = kChunkWaves * kRows * chunk_tiles((int)head_dim, dtype);
   p.chunk_tiles = 0;
   p.step_rows = INT32_MAX;
   // Chunks where their workgroups fill the card; the step kernel splits the keys where they do not.
@@ -1172,8 +1449,8 @@ void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     return;
   }
   if (p.chunk_tiles > 0)
-    hipLaunchKernelGGL((mx_attention_chunk_kernel<D, FMT, DT, kMost>),
-                       dim3((uint32_t)(p.chunk_tiles * a.kv_heads)), block, 0, st, a);
+    hipLaunchKernelGGL((mx_attention_chunk_kernel<D, FMT, DT, chunk_tiles(D, DT)>),
+                       dim3((uint32_t)(p.chunk_tiles * a.kv_heads)), dim3(kChunkWaves * 64), 0, st, a);
   if (p.query_tiles == 4) {
     if constexpr (kMost >= 4) hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 4>), steps, block, 0, st, a);
   } else if (p.query_tiles == 2) {
