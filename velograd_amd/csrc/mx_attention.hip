@@ -44,13 +44,15 @@ constexpr int chunk_parts(int dtype) {
   return dtype == VELOGRAD_DTYPE_BF16 ? 1 : dtype == VELOGRAD_DTYPE_F16 ? 2 : 3;
 }
 
-// Steps of a wave's share at least: one decode step over 2000 keys takes 12.2 us at 1, 11.0 at 2, 12.7 at 4, 14.6 at
-// 8 (fewer shares are joined faster, but last longer).
-// Query tiles of a wave of the chunk kernel, so that its rows, their sums and a step's scores fit 256 registers.
+// Query tiles of a wave of the chunk kernel, so that its rows, their sums and a step's scores fit 256 registers.  4096
+// new tokens of 6000, 32 heads, e2m1, at 1, 2 and 3 tiles: bf16 of 64 dims 262, 197 and (at 4) 320 us, of 128 dims 364,
+// 279 and 665, fp16 of 128 dims 465 and 391, fp32 of 64 dims 382, 336 and 460; of 256 dims 1 and 2 bf16 358 and 647.
 constexpr int chunk_tiles(int dim, int dtype) {
   return dim == 64 ? 2 : dim == 128 && dtype != VELOGRAD_DTYPE_F32 ? 2 : 1;
 }
 
+// Steps of a wave's share at least: one decode step over 2000 keys takes 12.2 us at 1, 11.0 at 2, 12.7 at 4, 14.6 at
+// 8 (fewer shares are joined faster, but last longer).
 constexpr int kLeastSteps = 2;
 // Steps that the beginning of an item counts for: 24 e4m3 sequences take 35.4 us at 0, 31.5 at 4, 30.7 at 6, 30.0 at
 // 10; 64 ragged ones 79.0, 77.5, 76.9 and 79.2.
@@ -1410,8 +1412,13 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
   const int64_t chunk_rows = kChunkWaves * kRows * chunk_tiles((int)head_dim, dtype);
   p.chunk_tiles = 0;
   p.step_rows = INT32_MAX;
-  // Chunks where their workgroups fill the card; the step kernel splits the keys where they do not.
-  if (ragged && q_tokens * q_heads >= chunk_rows * cus) {
+  // Chunks where their workgroups fill much of the card; the step kernel splits the keys where they do not, but decodes
+  // them for every wave.  32 heads of 128 dims, e2m1, new tokens of all, chunk and step kernel: bf16 512 of 8000 (a
+  // quarter of the card) 234 and 162 us, 1024 of 8000 (half) 235 and 262, 4 x 256 of 4000 129 and 168, 1536 of 8000 236
+  // and 392; fp16 1024 of 8000 354 and 264, 1536 of 8000 356 and 429; fp32 512 of 8000 (half) 281 and 216, 1024 of 8000
+  // 291 and 345.
+  const int64_t quarters = dtype == VELOGRAD_DTYPE_BF16 && chunk_tiles((int)head_dim, dtype) == 2 ? 2 : 3;
+  if (ragged && q_tokens * q_heads * 4 >= quarters * chunk_rows * cus) {
     p.chunk_tiles = q_tokens * group / chunk_rows + batch + 2;
     p.step_rows = kRows * 4;
   }
