@@ -11,8 +11,12 @@
 // K and V enter the products exactly, decoded by v_cvt_scalef32_pk_bf16_{fp4,fp8} in registers.  What is
 // not exact in bf16 is split into bf16 parts, each product summed in fp32: queries of bf16 are 1 part,
 // of fp16 2 (11 bits), of fp32 3 (24 bits), all exact; probabilities are rounded to 2 parts (off by at
-// most 2^-16, where the output's own half step is 2^-8 or 2^-11) and to 3 for fp32 outputs (2^-24).  Maxima,
-// sums and outputs are held in fp32.
+// most 2^-16, where the output's own half step is 2^-8 or 2^-11) and to 3 for fp32 outputs (2^-24); in chunks
+// of bf16 to 1 (chunk_parts).  Maxima, sums and outputs are held in fp32.
+//
+// Few rows are bound by the codes' bytes: the step kernel's waves each take an equal share of all keys and stream them
+// through LDS, and a second launch joins the pieces; where all is small, the item kernel does both.  Many rows are
+// bound by the products and the exponentials: the chunk kernel decodes keys once for all its waves.
 //
 // The products are laid out so that nothing crosses lanes.  A lane is (n = lane % 16, g = lane / 16).
 //   S^T = K Q^T: A = K, row n of half u of a 32-key tile is key 16 u + n; the contraction's order is free, so
@@ -38,8 +42,8 @@ constexpr int most_tiles(int dim, int dtype) {
   const int tiles = dtype == VELOGRAD_DTYPE_BF16 || dtype == VELOGRAD_DTYPE_F16 ? 4 : 2;
   return dim == 256 ? (dtype == VELOGRAD_DTYPE_BF16 ? 2 : 1) : dim == 128 && dtype == VELOGRAD_DTYPE_F16 ? 2 : tiles;
 }
-// Parts of a probability in chunks: the products count there, and one part of 8 bits (off by at most 2^-8 of
-// each probability, which average out over the keys) is as exact as the bf16 output.
+// Parts of a probability in chunks: the products count there, and one part of 8 bits is off by at most 2^-8 of each
+// probability, the half step that the bf16 output is rounded by anyway.
 constexpr int chunk_parts(int dtype) {
   return dtype == VELOGRAD_DTYPE_BF16 ? 1 : dtype == VELOGRAD_DTYPE_F16 ? 2 : 3;
 }
@@ -860,6 +864,10 @@ constexpr int step_occupancy(int dim, int fmt, int dtype, int query_tiles) {
   return dim < 256 || (small && dtype != VELOGRAD_DTYPE_F32) ? 2 : 1;
 }
 
+// A wave takes its share of a head's steps: whole items, and at either end a piece of one.  Bound by HBM: e2m1, bf16, 8
+// kv heads of 128 dims, 2 sequences of 131072 keys 56.7 us = 5.0 TB/s of codes and scales (a kernel that only reads
+// them so 47.6), 64 sequences of 300 to 12001 76.6 us = 5.6 TB/s.  Loads straight into registers, a tile ahead, took 71
+// and 95; scales read past the caches 57 and 80.
 template <int D, int FMT, int DT, int NQ>
 __global__ __launch_bounds__(kWaves * 64, step_occupancy(D, FMT, DT, NQ)) void mx_attention_step_kernel(const AttnArgs a) {
   using S = Shape<D, FMT, DT>;
@@ -1001,7 +1009,11 @@ __global__ __launch_bounds__(item_waves(D, FMT) * 64) void mx_attention_item_ker
 // A workgroup takes 128 NQ consecutive rows of one kv head over all the keys they see, a wave 16 NQ of them.  All
 // waves decode a step's keys together, a thread 16 elements of a key and 4 dims of 4 values, into LDS in the order
 // of the products' operands; each step's codes are loaded a step before they are decoded, so one barrier a step is
-// left.  The row tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
+// left.  Bound by instructions: matrix products and vector work (an exponential for each score, the decoding, the
+// operands' way out of LDS) add up more than they overlap on a SIMD.  4096 new tokens of 16383, 32 heads of 128 dims,
+// bf16: 830 us a pass = 1.16 PFLOP/s; in a kernel trace 1022 us, where decoding in every wave for itself (64 rows a wave,
+// one wave a SIMD) took 1112, a maximum taken in every step 1103 for 1086, waves half a step apart 1083 and 4 waves of 64
+// rows 1462.  The row tiles of one head go to one XCD where the heads divide so.  Later tiles see more keys and go first.
 constexpr int kChunkWaves = 8;
 
 // The codes of a thread's keys and values of one step.

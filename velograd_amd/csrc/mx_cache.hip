@@ -5,8 +5,8 @@
 //   codes   [pages, kv_heads, page_size, R]
 //   scales  [pages, kv_heads, head_dim / 32, page_size]
 // A token's slot is page * page_size + place.  A head's vectors of consecutive tokens are contiguous,
-// so the attention reads whole lines; its scales lie token by token, so the 8 scales that a lane needs
-// of 8 consecutive tokens are one 8-byte load.
+// so the attention reads whole lines; its scales lie token by token, so those of the 4 consecutive tokens
+// that a lane takes are one word.
 //
 // Quantisation is the norms' MX epilogue: per 32 elements a = max|x|, s = floor(log2 a) - emax clamped
 // to [-127, 127], codes RNE(x * 2^-s) saturating, scale code s + 127; a block whose maximum is not
@@ -19,7 +19,9 @@
 // would give.  A position outside the table rotates by NaN: the query row is NaN and the key's blocks
 // are marked NaN.
 //
-// Both kernels are bound by HBM (a few operations for each element).
+// Both kernels are bound by HBM (a few operations for each element): rotating and writing 8191 tokens (bf16, e2m1, 32
+// query and 8 kv heads of 128 dims) takes 38.6 us = 4.7 TB/s, reading 66000 tokens back 58.8 us = 5.8 TB/s.  Small
+// calls are bound by their launches: 8 tokens 3.5 us written, 2.6 read.
 #include "mx_device.h"
 
 namespace {

@@ -297,6 +297,9 @@ def mx_cache_attention(q: torch.Tensor, cache: MXCache, block_table: torch.Tenso
     the sum of exp(scale q.k) over the keys seen (to join with attention over other keys).  A row that sees
     no key, and a row of q past the last sequence, gives 0 and -inf.  Keys on a page outside the cache are
     not seen.
+
+    Scores, sums and outputs are held in float32.  Of a call with many rows in bfloat16 the probabilities are
+    rounded to bfloat16 (2^-8) before they multiply the values, elsewhere to 2^-16 or less.
     """
     fp = _fast(cache, q, block_table, lengths, *(() if q_starts is None else (q_starts,)))
     if fp is not None and q.dim() == 3:
