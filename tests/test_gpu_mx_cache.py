@@ -424,6 +424,25 @@ def test_lengths_past_the_table_and_below_zero_are_clamped():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_falling_starts_leave_the_buffers_alone():
+    """Outside the contract: rows are unspecified, but nothing past the buffers is touched."""
+    _say("falling starts")
+    rng = np.random.default_rng(31)
+    lengths = [300 + 5 * i for i in range(90)]
+    for tokens, heads in ((180, 8), (2100, 32)):              # the step kernel's call, the chunk kernel's
+        fresh = [tokens // 90] * 90
+        fresh[0] += tokens - sum(fresh)
+        parts, table, starts, q = _setup(rng, torch.bfloat16, "e2m1", 64, heads, 2, 16, lengths, fresh, 0, 70000)
+        want = _attend(q, parts, table, lengths, starts, "e2m1")
+        bad = starts.copy()
+        bad[1::2], bad[2::2] = tokens, 0
+        out, lse = _attend(q, parts, table, lengths, bad, "e2m1")
+        torch.cuda.synchronize()
+        assert out.shape == q.shape and lse.shape == q.shape[:2]
+        again = _attend(q, parts, table, lengths, starts, "e2m1")
+        assert torch.equal(want[0], again[0]) and torch.equal(want[1], again[1])
+
+
 def test_empty_calls():
     _say("empty calls")
     cache = vk.mx_cache(2, 16, 2, 64, "e4m3")

@@ -134,6 +134,12 @@ __device__ inline RowTile sequence_rows(const AttnArgs& a, int32_t i) {
   return r;
 }
 
+// Whether q_starts falls behind sequence i: no call that the entry point's contract allows.  The kernels then leave rows
+// out, but stay inside their buffers: a share's steps are counted in 32 bits, which only disjoint rows cannot exceed.
+__device__ __forceinline__ bool falls(const AttnArgs& a, int32_t i) {
+  return a.starts != nullptr && i < sequences(a) && row_bound(a, i + 1) < row_bound(a, i);
+}
+
 // Keys that new token i of the tile's sequence sees.
 __device__ inline int32_t row_limit(const AttnArgs& a, const RowTile& r, int32_t i) {
   int32_t x = a.causal ? r.length - r.fresh + i + 1 : r.length;
@@ -643,11 +649,16 @@ __device__ __forceinline__ Share find_share(const AttnArgs& a, int32_t tile_rows
   int32_t mine = sequence_steps(a, r, tile_rows);
   int32_t upto = wave_scan(mine);
   int32_t total = __builtin_amdgcn_readlane(upto, 63);
+  bool fall = falls(a, lane);
   if (count > 64) {
     int32_t more = 0;
-    for (int32_t i = lane + 64; i < count; i += 64) more += sequence_steps(a, sequence_rows(a, i), tile_rows);
+    for (int32_t i = lane + 64; i < count; i += 64) {
+      more += sequence_steps(a, sequence_rows(a, i), tile_rows);
+      fall |= falls(a, i);
+    }
     total += __builtin_amdgcn_readlane(wave_scan(more), 63);
   }
+  if (__ballot(fall) != 0) total = 0;
   const int32_t shares = a.workers / a.kv_heads;  // of a head
   Share s;
   s.each = (int32_t)(((uint32_t)total + (uint32_t)shares - 1) / (uint32_t)shares);
@@ -1364,10 +1375,14 @@ __global__ __launch_bounds__(256) void mx_attention_join_kernel(const AttnArgs a
   __syncthreads();
   for (int32_t k = 0; k < count; ++k) {
     const int64_t orow = blockIdx.x + (int64_t)found[k] * gridDim.x;
-    const int32_t first = a.joins[orow * 2], packed = a.joins[orow * 2 + 1];
-    const int32_t active = packed >> 8;
+    // In bounds whatever rows that no kernel took left there (falls).
+    const int32_t packed = a.joins[orow * 2 + 1];
+    int32_t first = a.joins[orow * 2], in_tile = packed & 0xff;
+    first = first < 0 ? 0 : first < a.workers ? first : a.workers - 1;
+    in_tile = in_tile < tile_rows ? in_tile : tile_rows - 1;
+    const int32_t most = (a.workers - 1 - first) / a.kv_heads + 1, active = packed >> 8 < most ? packed >> 8 : most;
     auto place = [&](int32_t s) {
-      return ((int64_t)(first + s * a.kv_heads) * 2 + (s == 0 ? 1 : 0)) * tile_rows + (packed & 0xff);
+      return ((int64_t)(first + s * a.kv_heads) * 2 + (s == 0 ? 1 : 0)) * tile_rows + in_tile;
     };
     float m = -3.0e38f;
     for (int32_t s = tid; s < active; s += 256) m = __builtin_fmaxf(m, a.part_ml[place(s) * 2]);

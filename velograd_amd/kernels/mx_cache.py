@@ -289,7 +289,7 @@ def mx_cache_attention(q: torch.Tensor, cache: MXCache, block_table: torch.Tenso
     query head h reads kv head h // (heads // kv_heads).  block_table, int32 [sequences, pages], lists each
     sequence's pages in order, lengths, int32 [sequences], the tokens it holds, its new ones included.
     q_starts, int32 [sequences + 1] rising from 0, says which rows of q are its new tokens
-    (q_starts[b] .. q_starts[b + 1] - 1); None: one each.  With causal, the i-th of n new tokens of a
+    (q_starts[b] .. q_starts[b + 1] - 1; where it falls, rows are left unset); None: one each.  With causal, the i-th of n new tokens of a
     sequence of L sees the first L - n + i + 1 keys, without, all L.  scale defaults to
     1 / sqrt(head_dim).
 
