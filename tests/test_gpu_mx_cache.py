@@ -324,6 +324,38 @@ def test_chunks_keep_nan_values_from_rows_that_do_not_see_them():
     assert torch.equal(out[..., :32], clean[0][..., :32])
 
 
+@pytest.mark.parametrize("dtype,dim,heads", [("bf16", 128, 16), ("fp16", 64, 24), ("fp32", 256, 16)])
+def test_chunks_with_missing_pages_and_nan_codes(dtype, dim, heads):
+    """From a missing page on, a chunk's steps are masked; e4m3 has NaN codes of single elements."""
+    _say(f"chunks bad pages {dtype} {dim}")
+    rng = np.random.default_rng(dim)
+    lengths, fresh = [2500, 31, 400], [2450, 2, 390]
+    parts, table, starts, q = _setup(rng, DTYPES[dtype], "e4m3", dim, heads, 1, 16, lengths, fresh, 3)
+    table[0, 3], table[0, 60], table[0, 101:103], table[2, :2] = -1, parts[0].shape[0], 1 << 30, -(1 << 31)
+    got = _attend(q, parts, table, lengths, starts, "e4m3")
+    _check(got, q, parts, table, lengths, starts, 16, "e4m3", p_eps=CHUNK_P_EPS[DTYPES[dtype]])
+    at = 1234
+    parts[2][table[0, at // 16], 0, at % 16, 5] = 0xff
+    out, lse = _attend(q, parts, table, lengths, starts, "e4m3")
+    first = at - (2500 - 2450)
+    assert torch.isnan(out[first:2450, :, 5]).all() and torch.equal(lse, got[1])
+    out[first:2450, :, 5] = got[0][first:2450, :, 5]
+    assert torch.equal(out, got[0])
+    parts[0][table[0, at // 16], 0, at % 16, 7] = 0x7f                  # a key: whole rows
+    out, lse = _attend(q, parts, table, lengths, starts, "e4m3")
+    assert torch.isnan(out[first:2450]).all() and torch.isnan(lse[first:2450]).all()
+    assert torch.equal(out[:first], got[0][:first]) and torch.equal(out[2450:], got[0][2450:])
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0, -0.3])
+def test_chunks_scales(scale):
+    _say(f"chunks scale {scale}")
+    rng = np.random.default_rng(41)
+    parts, table, starts, q = _setup(rng, torch.bfloat16, "e2m1", 64, 32, 2, 32, [1300, 70], [1290, 5], 0)
+    got = _attend(q, parts, table, [1300, 70], starts, "e2m1", scale=scale)
+    _check(got, q, parts, table, [1300, 70], starts, 32, "e2m1", scale=scale, p_eps=CHUNK_P_EPS[torch.bfloat16])
+
+
 @pytest.mark.usefixtures("table_room")
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_attention_scales(scale):
@@ -547,12 +579,13 @@ def test_a_layer_of_a_larger_allocation_and_strided_index_tensors():
     assert torch.equal(got, want[0])
 
 
-def test_captured_and_replayed_between_eager_calls():
-    _say("graphs")
+@pytest.mark.parametrize("each", [200, 60])   # pages of a sequence: split over the keys, in one launch
+def test_captured_and_replayed_between_eager_calls(each):
+    _say(f"graphs {each}")
     rng = np.random.default_rng(15)
     heads, kv, dim, page, fmt, seqs = 8, 2, 128, 16, "e2m1", 3
     cos_sin = vk.rope_table(4000, dim)
-    pages = 3 * 200
+    pages = 3 * each
     cache = vk.mx_cache(pages, page, kv, dim, fmt)
     eager = vk.mx_cache(pages, page, kv, dim, fmt)
     base = _randn(rng, (pages * page, 2 * kv, dim), torch.bfloat16)
@@ -580,7 +613,7 @@ def test_captured_and_replayed_between_eager_calls():
             outs.append(step(cache))
         graphs.append(g)
     for n in range(6):
-        at = [(700 * n + 1000 * i) % 3100 for i in range(seqs)]
+        at = [(700 * n + 1000 * i) % (each * page - 100) for i in range(seqs)]
         x.copy_(_randn(rng, x.shape, torch.bfloat16))
         pos.copy_(torch.tensor(at))
         held.copy_(torch.tensor(at, dtype=torch.int32) + 1)
@@ -593,6 +626,31 @@ def test_captured_and_replayed_between_eager_calls():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), n
         for a, b in zip(cache, eager):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), n
+
+
+def test_chunks_captured_with_other_lengths():
+    """A captured call takes its sequences' rows and lengths from device memory at each replay."""
+    _say("chunks graph")
+    rng = np.random.default_rng(43)
+    parts, table, starts, q = _setup(rng, torch.bfloat16, "e2m1", 64, 32, 4, 16, [1500, 900, 40], [1200, 60, 20], 40)
+    cache = R.from_bytes(parts, "e2m1", "cuda")
+    t = torch.from_numpy(table).cuda()
+    held = torch.tensor([1500, 900, 40], dtype=torch.int32, device="cuda")
+    at = torch.from_numpy(starts).cuda()
+    vk.mx_cache_attention(q, cache, t, held, at, return_lse=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = vk.mx_cache_attention(q, cache, t, held, at, return_lse=True)
+    for new, lens in (([1200, 60, 20], [1500, 900, 40]), ([1, 1, 1], [1500, 3, 0]), ([0, 890, 30], [700, 900, 35]),
+                      ([1310, 2, 0], [1400, 17, 16])):
+        held.copy_(torch.tensor(lens, dtype=torch.int32))
+        at.copy_(torch.tensor(np.concatenate(([0], np.cumsum(new))), dtype=torch.int32))
+        graph.replay()
+        want = vk.mx_cache_attention(q, cache, t, held, at, return_lse=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), (new, lens)
+        assert (out[sum(new):] == 0).all() and torch.isneginf(lse[sum(new):]).all()
 
 
 def test_streams():
