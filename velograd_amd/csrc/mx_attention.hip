@@ -1459,12 +1459,17 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
   if (p.workers < kv_heads) p.workers = (int32_t)((kv_heads + kWaves - 1) / kWaves * kWaves);
   p.least_steps = kLeastSteps;
   p.begin_steps = kBeginSteps;
-  // One launch, where the card has room for all items at once and a wave's run of the keys is short: the second
-  // launch costs 4 us, a run of 128 keys of 128 dims as much.  With more items the split's shares grow as well.  One
-  // sequence, 8 kv heads: 500 keys 11.0 us split and 8.1 in one launch, 1000 11.6 and 10.7, 2000 11.5 and 14.8;
-  // 16 sequences: 500 keys 14.7 and 8.9, 2000 20.1 and 15.6, 4000 25.5 and 24.1.
+  // One launch, where the card takes all items in few turns and a wave's run of the keys is short: the second launch
+  // costs 4 us, a run of 128 keys of 128 dims as much.  With more items the split's shares grow as well, and with several
+  // row tiles a sequence so do its pieces.  One sequence, 8 kv heads: 500 keys 11.0 us split and 8.1 in one launch,
+  // 1000 11.6 and 10.7, 2000 11.5 and 14.8; 16 sequences: 500 keys 14.7 and 8.9, 2000 20.1 and 15.6; 64: 2000 37.8 and
+  // 35.1; 128: 1000 43.9 and 47.7.  Rows of 36 tokens of 8 sequences of 1348 keys 68.5 and 38.8, of 128 tokens of 2 of
+  // 6000 97.8 and 63.2; 8 tokens of 32 of 2000, 2 kv heads of 256 e4m3 dims, 71.7 and 77.9.
+  const bool wide = rows > kRows;
   const int64_t items = (ragged ? q_tokens * group / kRows + batch + 2 : batch * ((group + kRows - 1) / kRows)) * kv_heads;
-  p.items = items <= cus && table_keys * head_dim <= item_waves((int)head_dim, fmt) * 128 * (128 + items) ? items : 0;
+  const int64_t wave_keys = 128 + (wide ? 2 * items : items < cus ? items : cus);
+  const bool short_runs = table_keys * head_dim <= item_waves((int)head_dim, fmt) * 128 * wave_keys;
+  p.items = p.chunk_tiles == 0 && items <= (wide ? 4 : 2) * cus && short_runs ? items : 0;
   return p;
 }
 
