@@ -1463,8 +1463,8 @@ AttnPlan plan_attention(int64_t q_tokens, int64_t batch, int64_t q_heads, int64_
   // costs 4 us, a run of 128 keys of 128 dims as much.  With more items the split's shares grow as well, and with several
   // row tiles a sequence so do its pieces.  One sequence, 8 kv heads: 500 keys 11.0 us split and 8.1 in one launch,
   // 1000 11.6 and 10.7, 2000 11.5 and 14.8; 16 sequences: 500 keys 14.7 and 8.9, 2000 20.1 and 15.6; 64: 2000 37.8 and
-  // 35.1; 128: 1000 43.9 and 47.7.  Rows of 36 tokens of 8 sequences of 1348 keys 68.5 and 38.8, of 128 tokens of 2 of
-  // 6000 97.8 and 63.2; 8 tokens of 32 of 2000, 2 kv heads of 256 e4m3 dims, 71.7 and 77.9.
+  // 35.1; 128: 1000 43.9 and 47.7.  Rows of 36 tokens of 8 sequences of 1348 keys 53.8 and 38.8, of 128 tokens of 2 of
+  // 6000 78.9 and 63.2; 8 tokens of 32 of 2000, 2 kv heads of 256 e4m3 dims, 71.7 and 77.9.
   const bool wide = rows > kRows;
   const int64_t items = (ragged ? q_tokens * group / kRows + batch + 2 : batch * ((group + kRows - 1) / kRows)) * kv_heads;
   const int64_t wave_keys = 128 + (wide ? 2 * items : items < cus ? items : cus);
@@ -1498,7 +1498,9 @@ void launch_attention(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     hipLaunchKernelGGL((mx_attention_step_kernel<D, FMT, DT, 1>), steps, block, 0, st, a);
   }
   const int64_t all = (int64_t)a.q_tokens * a.q_heads;
-  const int64_t rows = all <= 4096 ? 1 : all <= 16 * 4096 ? 16 : 256;
+  // Of 288 tokens of 32 heads all rows are joined: 53.8 us a call at one row a workgroup, 68.7 at 16.  Of 6216 of 32, a
+  // hundredth: 5.8 us in the join at 64, 7.6 at 16.
+  const int64_t rows = all <= 16384 ? 1 : all <= 65536 ? 4 : all <= 262144 ? 64 : 256;
   hipLaunchKernelGGL((mx_attention_join_kernel<D, DT>), dim3((uint32_t)((all + rows - 1) / rows)), dim3(256), 0, st,
                      a, kRows * p.query_tiles, (int32_t)rows);
 }
