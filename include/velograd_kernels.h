@@ -349,7 +349,8 @@ VELOGRAD_API int32_t velograd_mx_cache_read(
  *                 order.  Keys on a page outside the cache are not seen.
  *   lengths     : int32 [sequences], tokens that each sequence holds (clamped to 0 .. table_width * page_size).
  *   q_starts    : int32 [sequences + 1], rising from 0: sequence b's new tokens are rows q_starts[b] ..
- *                 q_starts[b + 1] - 1 of q.  NULL: one for each sequence (q_tokens == sequences).
+ *                 q_starts[b + 1] - 1 of q.  Where they fall, rows are left unset.  NULL: one
+ *                 for each sequence (q_tokens == sequences).
  *   causal      : nonzero: the i-th of n new tokens of a sequence of L sees its first L - n + i + 1 keys;
  *                 zero: all L.
  *   out         : [q_tokens, q_heads, head_dim] in `dtype`, contiguous, 16-byte aligned.
